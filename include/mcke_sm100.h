@@ -356,6 +356,88 @@ typedef struct {
 int mcke_sm100_gemm_plan(int64_t m, int64_t n, int64_t k, int variant, int c_dtype, int sm_count,
                          mcke_gemm_plan* out);
 
+/* ---- operators of language models (no counterpart in the reference) ------------
+ *
+ * Rows of float32 or bfloat16 (`dtype`: mcke_dtype), the last dimension
+ * contiguous, rows `*_stride` elements apart (any alignment of the element's own
+ * size; an input's rows may repeat, stride 0, an output's may not overlap).
+ * Weights, biases, statistics and log probabilities are float32; sums and
+ * statistics are never held in fewer than 32 bits.  No output may share a byte
+ * with an input or another output unless said otherwise (two column windows of
+ * one buffer do not).  A workspace is written before it is read, need not be
+ * cleared and must not be shared by calls that may run at the same time (two
+ * captured graphs on two streams, for instance).  Results have the same bits on
+ * every run.  All calls may be captured into a CUDA graph.  The stream belongs to
+ * the current device. */
+
+/* Layer norm of each row: y = (x - mean) * rstd * weight + bias with
+ * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  weight and bias: [cols] or NULL
+ * (1 and 0).  mean and rstd: [rows], what the backward pass takes, or NULL.
+ * eps finite and >= 0. */
+int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const float* weight, const float* bias, void* y,
+                          int64_t y_stride, float* mean, float* rstd, int64_t rows, int64_t cols, float eps,
+                          int dtype, mcke_stream_t stream);
+/* The backward pass.  With xh = (x - mean) * rstd and g = dy * weight:
+ * dx = rstd * (g - mean(g) - xh * mean(g * xh)), dweight = the sum over rows of
+ * dy * xh, dbias = the sum over rows of dy.  dweight and dbias: [cols] or NULL
+ * (with both NULL no workspace is needed).  rows == 0 writes zeros to them. */
+size_t mcke_sm100_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
+                                   const float* weight, const float* mean, const float* rstd, void* dx,
+                                   int64_t dx_stride, float* dweight, float* dbias, int64_t rows, int64_t cols,
+                                   int dtype, void* workspace, size_t workspace_bytes, mcke_stream_t stream);
+
+/* Of each row of logits: logprobs = the log probability of its target,
+ * lse = log(sum(exp)), entropy = -sum(p log p) (natural logarithms), and the
+ * top_k likeliest tokens (top_logprobs, top_ids: [rows, top_k], 0 .. MCKE_TOP_MAX
+ * of them, by value and among equals by index; NaN above all).  Any of the
+ * outputs may be NULL (top_k 0).
+ * A logit of -inf is a token that cannot come.  A row with nothing else has
+ * lse, logprobs and top_logprobs -inf and entropy 0.  A NaN or a +inf makes the
+ * row's results NaN.  A negative target is padding: log probability 0.  A target
+ * >= cols gives NaN. */
+#define MCKE_TOP_MAX 32
+int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int64_t rows, int64_t cols, int dtype,
+                              const int64_t* targets, float* logprobs, float* lse, float* entropy, int top_k,
+                              float* top_logprobs, int64_t* top_ids, mcke_stream_t stream);
+/* dlogits of the same rows, from the gradients of logprobs, entropy and lse (any
+ * of them NULL, not all): with p = exp(logits - lse),
+ * dlogits_j = grad_logprobs * ([j = target] - p_j)
+ *             - grad_entropy * p_j * (log p_j + entropy) + grad_lse * p_j.
+ * lse and entropy are the forward pass's (entropy only with grad_entropy,
+ * targets only with grad_logprobs).  A row of -inf alone gets zeros; a negative
+ * target takes no part in grad_logprobs, one >= cols gives NaN.  dlogits may be
+ * logits itself (same pointer, same stride). */
+int mcke_sm100_token_logprobs_backward(const void* logits, int64_t stride, int64_t rows, int64_t cols, int dtype,
+                                       const float* lse, const int64_t* targets, const float* grad_logprobs,
+                                       const float* entropy, const float* grad_entropy, const float* grad_lse,
+                                       void* dlogits, int64_t dlogits_stride, mcke_stream_t stream);
+
+/* One contiguous tensor of a gradient list (host array; read before the call
+ * returns).  out: where the clipped gradient goes, `data` itself to clip in
+ * place; its type is the gradient's or float32.  grad_norm ignores out. */
+typedef struct {
+  const void* data;
+  void* out;
+  int64_t numel;
+  int dtype;
+  int out_dtype;
+} mcke_grad;
+/* norm = sqrt of the sum of squares of every element of the list (one float,
+ * device memory; squares are added in double; 0 for an empty list). */
+size_t mcke_sm100_grad_norm_workspace_bytes(int count);
+int mcke_sm100_grad_norm(const mcke_grad* grads, int count, float* norm, void* workspace, size_t workspace_bytes,
+                         mcke_stream_t stream);
+/* out = min(1, max_norm / (norm + 1e-6)) * data for every tensor, the norm given
+ * in device memory (of several ranks' shards: the root of the sum of their
+ * squares).  A NaN norm makes the outputs NaN.  An output may share bytes with no
+ * other tensor of the list.  max_norm finite and >= 0. */
+int mcke_sm100_clip_grads(const mcke_grad* grads, int count, float max_norm, const float* norm,
+                          mcke_stream_t stream);
+/* Both: norm is written, and the list clipped by it. */
+int mcke_sm100_clip_grad_norm(const mcke_grad* grads, int count, float max_norm, float* norm, void* workspace,
+                              size_t workspace_bytes, mcke_stream_t stream);
+
 /* ---- roofline denominators (replace bench/stream_triad.cu and bench/fma_peak.cu) ----
  * Measurement probes, timed by the caller: a = b + scalar * c (12 bytes per
  * element moved) and a = b (8 bytes per element) with 128-bit streaming loads

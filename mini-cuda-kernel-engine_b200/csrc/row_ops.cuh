@@ -1,0 +1,106 @@
+// row_ops.cuh -- what the operators over rows of f32 or bf16 tensors share:
+// element access, warp and block sums, and the argument checks of their entry
+// points (row strides, overlap of outputs with inputs).
+#pragma once
+
+#include <cmath>
+
+#include "mcke_common.cuh"
+
+namespace mcke_sm100 {
+
+// ---- host: argument checks ------------------------------------------------------
+
+inline std::size_t dtype_bytes(int dtype) { return dtype == MCKE_DTYPE_BF16 ? 2 : 4; }
+
+// A block of rows: `rows` runs of `row_bytes` bytes, `pitch` bytes apart.
+struct RowSpan {
+  const char* name;
+  const void* p;
+  int64_t rows, row_bytes, pitch;
+};
+inline RowSpan span_of(const char* name, const void* p, int64_t rows, int64_t cols, int64_t stride, std::size_t elem) {
+  return RowSpan{name, p, rows, cols * static_cast<int64_t>(elem), stride * static_cast<int64_t>(elem)};
+}
+inline RowSpan span_of(const char* name, const void* p, int64_t bytes) { return RowSpan{name, p, 1, bytes, bytes}; }
+
+// Whether two blocks share a byte.  Blocks of one pitch that lie in disjoint
+// column windows of the same buffer do not.
+inline bool spans_overlap(const RowSpan& a, const RowSpan& b) {
+  if (!a.p || !b.p || a.rows <= 0 || b.rows <= 0 || a.row_bytes <= 0 || b.row_bytes <= 0) return false;
+  const auto a0 = reinterpret_cast<std::uintptr_t>(a.p), b0 = reinterpret_cast<std::uintptr_t>(b.p);
+  const std::uintptr_t a1 = a0 + static_cast<std::uintptr_t>((a.rows - 1) * a.pitch + a.row_bytes);
+  const std::uintptr_t b1 = b0 + static_cast<std::uintptr_t>((b.rows - 1) * b.pitch + b.row_bytes);
+  if (a1 <= b0 || b1 <= a0) return false;
+  if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch && a.pitch > 0) {
+    const std::uintptr_t pitch = static_cast<std::uintptr_t>(a.pitch);
+    const std::uintptr_t off = a0 <= b0 ? (b0 - a0) % pitch : (pitch - (a0 - b0) % pitch) % pitch;
+    // b's window starts `off` bytes after a's: behind a's end, and its end before a's next row
+    if (off >= static_cast<std::uintptr_t>(a.row_bytes) && off + static_cast<std::uintptr_t>(b.row_bytes) <= pitch)
+      return false;
+  }
+  return true;
+}
+
+// Every output against every input and every other output.
+template <int NOut, int NIn>
+inline int check_overlaps(const char* who, const RowSpan (&out)[NOut], const RowSpan (&in)[NIn]) {
+  for (int i = 0; i < NOut; ++i) {
+    for (int j = 0; j < NIn; ++j)
+      if (spans_overlap(out[i], in[j]))
+        return fail(MCKE_INVALID_ARGUMENT, "%s: %s overlaps %s", who, out[i].name, in[j].name);
+    for (int j = 0; j < i; ++j)
+      if (spans_overlap(out[i], out[j]))
+        return fail(MCKE_INVALID_ARGUMENT, "%s: %s overlaps %s", who, out[i].name, out[j].name);
+  }
+  return MCKE_OK;
+}
+
+inline int check_dtype(const char* who, int dtype) {
+  if (dtype != MCKE_DTYPE_F32 && dtype != MCKE_DTYPE_BF16)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: unknown dtype %d", who, dtype);
+  return MCKE_OK;
+}
+
+// Rows of an input may repeat or overlap (stride 0: one row read `rows` times);
+// rows of an output may not.
+inline int check_stride(const char* who, const char* name, int64_t stride, int64_t rows, int64_t cols, bool output) {
+  if (rows > 1 && (stride < 0 || (output && stride < cols)))
+    return fail(MCKE_INVALID_ARGUMENT, "%s: %s has row stride %lld for %lld columns", who, name,
+                static_cast<long long>(stride), static_cast<long long>(cols));
+  if (rows > 1 && stride > (int64_t{1} << 40) / rows)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: %s spans more than 2^40 elements", who, name);
+  return MCKE_OK;
+}
+
+// ---- device: elements ---------------------------------------------------------------
+
+// T is float, or uint16_t for raw bfloat16 patterns.
+__device__ __forceinline__ float ld_val(const float* p) { return *p; }
+__device__ __forceinline__ float ld_val(const uint16_t* p) { return from_bf16(*p); }
+__device__ __forceinline__ void st_val(float* p, float v) { *p = v; }
+__device__ __forceinline__ void st_val(uint16_t* p, float v) { *p = to_bf16(v); }
+
+// ---- device: sums --------------------------------------------------------------------
+
+template <class V>
+__device__ __forceinline__ V warp_all_sum(V v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// Sum over the block's `kWarps` warps, the same bits in every thread.  `red`:
+// kWarps values of shared memory that no thread still reads.
+template <int kWarps, class V>
+__device__ __forceinline__ V block_all_sum(V v, V* red) {
+  v = warp_all_sum(v);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
+  __syncthreads();
+  V t = red[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) t += red[w];
+  return t;
+}
+
+}  // namespace mcke_sm100

@@ -10,9 +10,11 @@ library is missing the first call raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import re
 import struct
+import typing
 
 import torch
 
@@ -100,6 +102,17 @@ def lib() -> ctypes.CDLL:
             "mcke_sm100_gemm_bf16_ex": (i32, [vp, vp, vp, i32, i64, i64, i64, f32, f32, vp, i32, i32, vp]),
             "mcke_sm100_gemm_kernel_attrs": (i32, [i32, i32, vp]),
             "mcke_sm100_gemm_plan": (i32, [i64, i64, i64, i32, i32, i32, vp]),
+            "mcke_sm100_layer_norm": (i32, [vp, i64, vp, vp, vp, i64, vp, vp, i64, i64, f32, i32, vp]),
+            "mcke_sm100_layer_norm_backward_workspace_bytes": (sz, [i64, i64]),
+            "mcke_sm100_layer_norm_backward": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, i64, i32, vp,
+                                                     sz, vp]),
+            "mcke_sm100_token_logprobs": (i32, [vp, i64, i64, i64, i32, vp, vp, vp, vp, i32, vp, vp, vp]),
+            "mcke_sm100_token_logprobs_backward": (i32, [vp, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64,
+                                                         vp]),
+            "mcke_sm100_grad_norm_workspace_bytes": (sz, [i32]),
+            "mcke_sm100_grad_norm": (i32, [vp, i32, vp, vp, sz, vp]),
+            "mcke_sm100_clip_grads": (i32, [vp, i32, f32, vp, vp]),
+            "mcke_sm100_clip_grad_norm": (i32, [vp, i32, f32, vp, vp, sz, vp]),
         }
         for name, (res, args) in sigs.items():
             fn = getattr(l, name)
@@ -482,6 +495,258 @@ def gemm_f32_tc(a, b, c=None, alpha: float = 1.0, beta: float = 0.0, bias=None, 
     _check(lib().mcke_sm100_gemm_f32_tc(_ptr(a), _ptr(b), _ptr(c), m, n, k, alpha, beta, _ptr(bias), _act(act),
                                         _ptr(workspace), workspace.numel(), _stream(a, stream)))
     return c
+
+
+# ---- operators of language models ----------------------------------------------------
+#
+# These calls run on the tensors' device whether or not it is the current one.
+# With an explicit ``stream`` what a call allocates belongs to that stream.
+
+_DTYPE_OF = {torch.float32: DTYPE["f32"], torch.bfloat16: DTYPE["bf16"]}
+
+
+def _rows_of(t: torch.Tensor, name: str, dtype=None) -> tuple[int, int, int]:
+    """(rows, cols, row stride) of a float32 or bfloat16 tensor: [rows, cols] with
+    any row stride, or any contiguous shape, rows over its last dimension."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.dtype not in _DTYPE_OF or (dtype is not None and t.dtype != dtype):
+        raise ValueError(f"{name} must be {dtype or 'float32 or bfloat16'}, got {t.dtype}")
+    if t.dim() == 2:
+        rows, cols = t.shape
+        if t.stride(1) == 1 or cols <= 1:
+            return rows, cols, t.stride(0)
+    elif t.dim() > 0 and t.is_contiguous():
+        cols = t.shape[-1]
+        return (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
+    raise ValueError(f"{name} must be [rows, cols] with contiguous rows, or contiguous")
+
+
+def _vector(t, n: int, dtype, name: str, like: torch.Tensor) -> int | None:
+    """Address of a contiguous vector of n elements on like's device (None stays None)."""
+    if t is None:
+        return None
+    if t.device != like.device:
+        raise ValueError(f"{name} must be on {like.device}, got {t.device}")
+    if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be {n} contiguous values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
+    return t.data_ptr()
+
+
+def _same(t, like: torch.Tensor, name: str) -> None:
+    if t.shape != like.shape or t.device != like.device:
+        raise ValueError(f"{name} must have shape {tuple(like.shape)} on {like.device}, got {tuple(t.shape)} on "
+                         f"{t.device}")
+
+
+class _On:
+    """The device and stream of one call: current inside the ``with``, so that
+    launches reach them and allocations belong to them.  Nothing is switched
+    where both are current already."""
+    __slots__ = ("handle", "_guards")
+
+    def __init__(self, device: torch.device, stream):
+        self._guards = []
+        if torch.cuda.current_device() != device.index:
+            self._guards.append(torch.cuda.device(device))
+        self.handle = torch.cuda.current_stream(device).cuda_stream
+        if stream is not None:
+            handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
+            if handle != self.handle:
+                if not hasattr(stream, "cuda_stream"):
+                    stream = torch.cuda.ExternalStream(handle, device=device)
+                self._guards.append(torch.cuda.stream(stream))
+                self.handle = handle
+
+    def __enter__(self) -> int:
+        for g in self._guards:
+            g.__enter__()
+        return self.handle
+
+    def __exit__(self, *exc):
+        for g in reversed(self._guards):
+            g.__exit__(*exc)
+
+
+def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, save_stats: bool = False, stream=None):
+    """Layer norm over the last dimension (mcke_sm100_layer_norm): x float32 or
+    bfloat16, weight and bias float32 [cols] or None.  Returns y, or (y, mean,
+    rstd) with ``save_stats``: the float32 row statistics that
+    :func:`layer_norm_backward` takes."""
+    rows, cols, xs = _rows_of(x, "x")
+    w, b = _vector(weight, cols, torch.float32, "weight", x), _vector(bias, cols, torch.float32, "bias", x)
+    if out is not None:
+        _same(out, x, "out")
+        ys = _rows_of(out, "out", x.dtype)[2]
+    with _On(x.device, stream) as s:
+        if out is None:
+            out, ys = torch.empty(x.shape, dtype=x.dtype, device=x.device), cols
+        mean = rstd = None
+        if save_stats:
+            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        _check(lib().mcke_sm100_layer_norm(x.data_ptr(), xs, w, b, out.data_ptr(), ys, _ptr(mean), _ptr(rstd), rows,
+                                           cols, eps, _DTYPE_OF[x.dtype], s))
+    return (out, mean, rstd) if save_stats else out
+
+
+def layer_norm_backward_workspace_bytes(rows: int, cols: int) -> int:
+    return lib().mcke_sm100_layer_norm_backward_workspace_bytes(rows, cols)
+
+
+def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None, param_grads: bool = True, workspace=None,
+                        stream=None):
+    """Gradients of :func:`layer_norm` (mcke_sm100_layer_norm_backward): (dx,
+    dweight, dbias), dx in x's type, the others float32 [cols]; only dx without
+    ``param_grads``."""
+    rows, cols, xs = _rows_of(x, "x")
+    _same(dy, x, "dy")
+    dys = _rows_of(dy, "dy", x.dtype)[2]
+    m, r = _vector(mean, rows, torch.float32, "mean", x), _vector(rstd, rows, torch.float32, "rstd", x)
+    w = _vector(weight, cols, torch.float32, "weight", x)
+    if out is not None:
+        _same(out, x, "out")
+        dxs = _rows_of(out, "out", x.dtype)[2]
+    if workspace is not None and workspace.device != x.device:
+        raise ValueError(f"workspace must be on {x.device}")
+    with _On(x.device, stream) as s:
+        if out is None:
+            out, dxs = torch.empty(x.shape, dtype=x.dtype, device=x.device), cols
+        dw = db = None
+        if param_grads:
+            dw, db = torch.empty((2, cols), dtype=torch.float32, device=x.device)
+            if workspace is None:
+                workspace = torch.empty(layer_norm_backward_workspace_bytes(rows, cols), dtype=torch.uint8,
+                                        device=x.device)
+        _check(lib().mcke_sm100_layer_norm_backward(
+            dy.data_ptr(), dys, x.data_ptr(), xs, w, m, r, out.data_ptr(), dxs, _ptr(dw), _ptr(db), rows, cols,
+            _DTYPE_OF[x.dtype], _ptr(workspace), 0 if workspace is None else workspace.nbytes, s))
+    return (out, dw, db) if param_grads else out
+
+
+TOP_MAX = 32  # MCKE_TOP_MAX
+
+
+class TokenLogprobs(typing.NamedTuple):
+    """What :func:`token_logprobs` found; None for what was not asked for."""
+    logprobs: torch.Tensor | None
+    lse: torch.Tensor
+    entropy: torch.Tensor | None
+    top_logprobs: torch.Tensor | None
+    top_ids: torch.Tensor | None
+
+
+def token_logprobs(logits, targets=None, top_k: int = 0, entropy: bool = False, stream=None) -> TokenLogprobs:
+    """Log probabilities under rows of logits (mcke_sm100_token_logprobs): of each
+    row's target (int64, one per row; negative: padding, 0), the log-sum-exp, the
+    entropy, and the ``top_k`` likeliest tokens (log probabilities and int64 ids).
+    Shapes are logits' without the last dimension (and [..., top_k])."""
+    rows, cols, xs = _rows_of(logits, "logits")
+    t = _vector(targets, rows, torch.int64, "targets", logits)
+    shape, dev = logits.shape[:-1], logits.device
+    with _On(dev, stream) as s:
+        n = 1 + (targets is not None) + bool(entropy)
+        vals = torch.empty((n, *shape), dtype=torch.float32, device=dev).unbind(0)
+        lse, lp, ent = vals[0], vals[1] if targets is not None else None, vals[-1] if entropy else None
+        top = ids = None
+        if top_k:
+            k = max(int(top_k), 0)  # the library refuses a negative one
+            top = torch.empty((*shape, k), dtype=torch.float32, device=dev)
+            ids = torch.empty((*shape, k), dtype=torch.int64, device=dev)
+        _check(lib().mcke_sm100_token_logprobs(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype], t, _ptr(lp),
+                                               lse.data_ptr(), _ptr(ent), top_k, _ptr(top), _ptr(ids), s))
+    return TokenLogprobs(lp, lse, ent, top, ids)
+
+
+def token_logprobs_backward(logits, lse, targets=None, grad_logprobs=None, entropy=None, grad_entropy=None,
+                            grad_lse=None, out=None, stream=None):
+    """The gradient of logits from those of :func:`token_logprobs`' logprobs,
+    entropy and lse (mcke_sm100_token_logprobs_backward), in logits' type.
+    ``out`` may be ``logits`` itself."""
+    rows, cols, xs = _rows_of(logits, "logits")
+    f = lambda v, name: _vector(v, rows, torch.float32, name, logits)  # noqa: E731
+    args = (f(lse, "lse"), _vector(targets, rows, torch.int64, "targets", logits), f(grad_logprobs, "grad_logprobs"),
+            f(entropy, "entropy"), f(grad_entropy, "grad_entropy"), f(grad_lse, "grad_lse"))
+    if out is not None:
+        _same(out, logits, "out")
+        ds = _rows_of(out, "out", logits.dtype)[2]
+    with _On(logits.device, stream) as s:
+        if out is None:
+            out, ds = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), cols
+        _check(lib().mcke_sm100_token_logprobs_backward(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype],
+                                                        *args, out.data_ptr(), ds, s))
+    return out
+
+
+class Grad(ctypes.Structure):
+    """mcke_grad: one tensor of a gradient list."""
+    _fields_ = [("data", ctypes.c_void_p), ("out", ctypes.c_void_p), ("numel", ctypes.c_int64),
+                ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
+
+
+def _grad_list(grads, outs):
+    """(mcke_grad array, count, device) of contiguous float32 and bfloat16 tensors."""
+    if not grads:
+        raise ValueError("the list of gradients is empty")
+    if len(outs) != len(grads):
+        raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
+    dev = grads[0].device
+    for kind, tensors in (("gradient", grads), ("output", outs)):
+        for i, t in enumerate(tensors):
+            if not t.is_cuda or t.device != dev or t.dtype not in _DTYPE_OF or not t.is_contiguous():
+                raise ValueError(f"{kind} {i} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
+    if outs is not grads:
+        for i, (g, o) in enumerate(zip(grads, outs)):
+            if g.shape != o.shape:
+                raise ValueError(f"output {i} must have shape {tuple(g.shape)}, got {tuple(o.shape)}")
+    arr = (Grad * len(grads))(*[(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE_OF[g.dtype], _DTYPE_OF[o.dtype])
+                                for g, o in zip(grads, outs)])
+    return arr, len(grads), dev
+
+
+def _norm_call(arr, n, dev, stream, norm, workspace, call):
+    with _On(dev, stream) as s:
+        if norm is None:
+            norm = torch.empty((), dtype=torch.float32, device=dev)
+        elif norm.device != dev or norm.dtype != torch.float32 or norm.numel() != 1:
+            raise ValueError(f"norm must be one float32 on {dev}")
+        if workspace is None:
+            workspace = torch.empty(grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        elif workspace.device != dev:
+            raise ValueError(f"workspace must be on {dev}")
+        _check(call(norm.data_ptr(), workspace.data_ptr(), workspace.nbytes, s))
+    return norm
+
+
+def grad_norm_workspace_bytes(count: int) -> int:
+    return lib().mcke_sm100_grad_norm_workspace_bytes(count)
+
+
+def grad_norm(grads, norm=None, workspace=None, stream=None):
+    """The L2 norm over every element of a list of contiguous float32 and bfloat16
+    tensors (mcke_sm100_grad_norm): one float32 on their device."""
+    arr, n, dev = _grad_list(grads, grads)
+    return _norm_call(arr, n, dev, stream, norm, workspace,
+                      lambda *a: lib().mcke_sm100_grad_norm(arr, n, *a))
+
+
+def clip_grad_norm(grads, max_norm: float, out=None, norm=None, workspace=None, stream=None):
+    """Scales the gradients by min(1, max_norm / (norm + 1e-6))
+    (mcke_sm100_clip_grad_norm), in place or into the tensors of ``out`` (the
+    gradients' types, or float32).  Returns the norm before clipping."""
+    arr, n, dev = _grad_list(grads, grads if out is None else out)
+    return _norm_call(arr, n, dev, stream, norm, workspace,
+                      lambda *a: lib().mcke_sm100_clip_grad_norm(arr, n, max_norm, *a))
+
+
+def clip_grads(grads, max_norm: float, norm, out=None, stream=None) -> None:
+    """:func:`clip_grad_norm` by a norm that the caller has on the device
+    (mcke_sm100_clip_grads): that of all ranks' gradients, for instance, which
+    is the root of the sum of the ranks' squared norms."""
+    arr, n, dev = _grad_list(grads, grads if out is None else out)
+    if norm.device != dev or norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError(f"norm must be one float32 on {dev}")
+    with _On(dev, stream) as s:
+        _check(lib().mcke_sm100_clip_grads(arr, n, max_norm, norm.data_ptr(), s))
 
 
 class GemmAttrs(ctypes.Structure):
