@@ -9,6 +9,9 @@
 // Statistics and sums are float whatever the tensors' type; y and dx are rounded
 // once.  The variance is the mean of the squared deviations from the row's
 // mean, not a difference of two large sums.
+#include <initializer_list>
+#include <type_traits>
+
 #include "row_ops.cuh"
 
 namespace mcke_sm100 {
@@ -17,7 +20,648 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
-// One block per row, three reads of it.
+// A thread's unit of a row: 16 bytes of it.
+template <class T>
+struct Unit;
+template <>
+struct Unit<float> {
+  static constexpr int kPer = 4;
+  static __device__ __forceinline__ uint4 load(const float* p) { return ld_stream_u4(p); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x);
+    v[1] = __uint_as_float(q.y);
+    v[2] = __uint_as_float(q.z);
+    v[3] = __uint_as_float(q.w);
+  }
+  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
+    st_stream_f4(p, make_float4(v[0], v[1], v[2], v[3]));
+  }
+  static __device__ __forceinline__ void pairs(const uint4& q, F2 (&v)[2]) {
+    v[0] = f2(__uint_as_float(q.x), __uint_as_float(q.y));
+    v[1] = f2(__uint_as_float(q.z), __uint_as_float(q.w));
+  }
+  static __device__ __forceinline__ void store_pairs(float* p, const F2 (&v)[2]) {
+    const float2 a = split(v[0]), b = split(v[1]);
+    st_stream_f4(p, make_float4(a.x, a.y, b.x, b.y));
+  }
+};
+template <>
+struct Unit<uint16_t> {
+  static constexpr int kPer = 8;
+  static __device__ __forceinline__ uint4 load(const uint16_t* p) { return ld_stream_u4(p); }
+  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[2 * j] = bf16_lo(w[j]);
+      v[2 * j + 1] = bf16_hi(w[j]);
+    }
+  }
+  static __device__ __forceinline__ void store(uint16_t* p, const float (&v)[8]) {
+    st_stream_u4(p, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                               pack_bf16x2(v[6], v[7])));
+  }
+  static __device__ __forceinline__ void pairs(const uint4& q, F2 (&v)[4]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = f2(bf16_lo(w[j]), bf16_hi(w[j]));
+  }
+  static __device__ __forceinline__ void store_pairs(uint16_t* p, const F2 (&v)[4]) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 a = split(v[j]);
+      w[j] = pack_bf16x2(a.x, a.y);
+    }
+    st_stream_u4(p, make_uint4(w[0], w[1], w[2], w[3]));
+  }
+};
+__device__ __forceinline__ uint4 no_unit() { return make_uint4(0u, 0u, 0u, 0u); }
+
+// kPer consecutive floats of a parameter vector (`other` where there is none).
+template <int kPer>
+__device__ __forceinline__ void load_param(const float* p, int c, float other, float (&v)[kPer]) {
+  if (!p) {
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) v[j] = other;
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPer; j += 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(p + c + j));
+      v[j] = f.x;
+      v[j + 1] = f.y;
+      v[j + 2] = f.z;
+      v[j + 3] = f.w;
+    }
+  }
+}
+
+// Blocks of a row kernel that are to fit an SM: its registers are held to that, or the
+// compiler keeps a row's parameters in flight and leaves no room for other rows.
+template <class T, int kUnits, int kRowWarps>
+struct RowBlocks {
+  static constexpr int kThreadsPer = kRowWarps == 1 ? kThreads : 32 * kRowWarps;
+  static constexpr int kRegs = Unit<T>::kPer * kUnits + 36;  // the row as floats, and the rest
+  static constexpr int kMin = 65536 / (kThreadsPer * kRegs) < 1 ? 1 : 65536 / (kThreadsPer * kRegs);
+};
+
+struct ForwardArgs {
+  const void* x;
+  int64_t x_stride;
+  const float* weight;
+  const float* bias;
+  void* y;
+  int64_t y_stride;
+  float* mean;
+  float* rstd;
+  int rows, cols;
+  float eps;
+};
+
+// kPer consecutive values of a parameter vector, in pairs.
+template <int kPer>
+__device__ __forceinline__ void load_param_pairs(const float* p, int c, float other, F2 (&v)[kPer / 2]) {
+  float f[kPer];
+  load_param<kPer>(p, c, other, f);
+#pragma unroll
+  for (int j = 0; j < kPer / 2; ++j) v[j] = f2(f[2 * j], f[2 * j + 1]);
+}
+
+// A row in the registers of kRowWarps warps, kUnits units a thread (a warp per row: eight
+// rows a block, no barrier; else a block per row): x is read once and y
+// written once.  The units stay packed, so a bf16 row of 4096 is 64 registers of
+// one warp.  kFull: the row fills the threads' units, and none needs a check.
+template <class T, int kUnits, int kRowWarps, bool kFull>
+__global__ void __launch_bounds__(kRowWarps == 1 ? kThreads : 32 * kRowWarps, RowBlocks<T, kUnits, kRowWarps>::kMin)
+    layer_norm_kernel(const ForwardArgs a) {
+  pdl_entry();
+  using U = Unit<T>;
+  constexpr int kPer = U::kPer, kPairs = kPer / 2;
+  __shared__ float red[2][kRowWarps];
+  const int t = kRowWarps == 1 ? threadIdx.x & 31 : threadIdx.x;
+  const int row = kRowWarps == 1 ? blockIdx.x * kWarps + (threadIdx.x >> 5) : blockIdx.x;
+  if (kRowWarps == 1 && row >= a.rows) return;
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_stride + t * kPer;
+  T* yr = static_cast<T*>(a.y) + row * a.y_stride + t * kPer;
+  constexpr int kStep = 32 * kRowWarps * kPer;
+  auto live = [&](int i) { return kFull || i * kStep + t * kPer < a.cols; };
+  uint4 q[kUnits];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) q[i] = live(i) ? U::load(xr + i * kStep) : no_unit();
+  F2 s2 = f2(0.0f);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    F2 v[kPairs];
+    U::pairs(q[i], v);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) s2 = add2(s2, v[j]);
+  }
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  const float s = kRowWarps == 1 ? warp_all_sum(sum2(s2)) : block_all_sum<kRowWarps>(sum2(s2), red[0]);
+  const float mu = div_by(s, n, inv_n);
+  const F2 minus_mu = f2(-mu);
+  F2 d2 = f2(0.0f);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (!live(i)) continue;
+    F2 v[kPairs];
+    U::pairs(q[i], v);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      v[j] = add2(v[j], minus_mu);
+      d2 = fma2(v[j], v[j], d2);
+    }
+  }
+  const float var = kRowWarps == 1 ? warp_all_sum(sum2(d2)) : block_all_sum<kRowWarps>(sum2(d2), red[1]);
+  const float r = rsqrtf(div_by(var, n, inv_n) + a.eps);
+  if (t == 0) {
+    if (a.mean) a.mean[row] = mu;
+    if (a.rstd) a.rstd[row] = r;
+  }
+  const F2 rr = f2(r);
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (!live(i)) continue;
+    F2 v[kPairs], w[kPairs], b[kPairs];
+    U::pairs(q[i], v);
+    load_param_pairs<kPer>(a.weight, i * kStep + t * kPer, 1.0f, w);
+    load_param_pairs<kPer>(a.bias, i * kStep + t * kPer, 0.0f, b);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) v[j] = fma2(mul2(add2(v[j], minus_mu), rr), w[j], b[j]);
+    U::store_pairs(yr + i * kStep, v);
+  }
+}
+
+// Rows that are not whole 16-byte units from a 16-byte boundary on: a block per row,
+// consecutive threads on consecutive elements, kPairs pairs of elements (of columns
+// c and c + kThr) to a thread.  The row fills all pairs but the last.
+template <class T, int kPairs, int kThr>
+__global__ void __launch_bounds__(kThr) layer_norm_elements_kernel(const ForwardArgs a) {
+  pdl_entry();
+  __shared__ float red[2][kThr / 32];
+  const int row = blockIdx.x;
+  const T* xr = static_cast<const T*>(a.x) + row * a.x_stride + threadIdx.x;
+  T* yr = static_cast<T*>(a.y) + row * a.y_stride + threadIdx.x;
+  const int left = a.cols - 2 * (kPairs - 1) * kThr - static_cast<int>(threadIdx.x);  // the last pair's: > 0, > kThr
+  auto lo_live = [&](int i) { return i + 1 < kPairs || left > 0; };
+  auto hi_live = [&](int i) { return i + 1 < kPairs || left > kThr; };
+  F2 v[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i)
+    v[i] = f2(lo_live(i) ? ld_val(xr + 2 * i * kThr) : 0.0f, hi_live(i) ? ld_val(xr + (2 * i + 1) * kThr) : 0.0f);
+  F2 s2 = v[0];
+#pragma unroll
+  for (int i = 1; i < kPairs; ++i) s2 = add2(s2, v[i]);
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  const float mu = div_by(block_all_sum<kThr / 32>(sum2(s2), red[0]), n, inv_n);
+  const F2 minus_mu = f2(-mu);
+  F2 d2 = f2(0.0f);
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    v[i] = add2(v[i], minus_mu);
+    const float2 d = split(v[i]);
+    const F2 counted = i + 1 < kPairs ? v[i] : f2(lo_live(i) ? d.x : 0.0f, hi_live(i) ? d.y : 0.0f);
+    d2 = fma2(counted, counted, d2);
+  }
+  const float r = rsqrtf(div_by(block_all_sum<kThr / 32>(sum2(d2), red[1]), n, inv_n) + a.eps);
+  if (threadIdx.x == 0) {
+    if (a.mean) a.mean[row] = mu;
+    if (a.rstd) a.rstd[row] = r;
+  }
+  const F2 rr = f2(r);
+  auto finish = [&](auto weight, auto bias) {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) {
+      const int c = 2 * i * kThr + threadIdx.x;
+      const F2 w = f2(lo_live(i) ? weight(c) : 0.0f, hi_live(i) ? weight(c + kThr) : 0.0f);
+      const F2 b = f2(lo_live(i) ? bias(c) : 0.0f, hi_live(i) ? bias(c + kThr) : 0.0f);
+      const float2 y = split(fma2(mul2(v[i], rr), w, b));
+      if (lo_live(i)) st_val(yr + 2 * i * kThr, y.x);
+      if (hi_live(i)) st_val(yr + (2 * i + 1) * kThr, y.y);
+    }
+  };
+  auto w_at = [&](int c) { return __ldg(a.weight + c); };
+  auto b_at = [&](int c) { return __ldg(a.bias + c); };
+  auto one = [](int) { return 1.0f; };
+  auto zero = [](int) { return 0.0f; };
+  if (a.weight && a.bias) finish(w_at, b_at);
+  else if (a.weight) finish(w_at, zero);
+  else if (a.bias) finish(one, b_at);
+  else finish(one, zero);
+}
+
+// ---- rows streamed through shared memory ----------------------------------------
+//
+// A persistent block per SM of kGroups groups of kWarps warps; a group works on a
+// row at a time and a thread on the same kUnits 16-byte units of every row, so
+// the parameters (and the backward pass's column sums) stay in its registers.
+// Rows come through a ring of kStages in shared memory filled by asynchronous
+// copies: a thread copies only what it will read itself, so the ring needs no
+// barrier, and rows ahead are in flight while a row is worked on.
+template <class T, int kUnits, int kWarps, int kGroups, int kStages, int kOperands>
+struct Stream {
+  static constexpr int kTpg = 32 * kWarps;
+  static constexpr int kThreads = kTpg * kGroups;
+  static constexpr std::size_t kSmem = static_cast<std::size_t>(kStages) * kOperands * kUnits * kThreads * 16;
+  static_assert(kGroups <= 15, "a named barrier per group, besides the block's");
+};
+
+__device__ __forceinline__ void copy_unit_async(const uint4* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(static_cast<uint32_t>(__cvta_generic_to_shared(dst))),
+               "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// Sums over a group of kW warps (of each of the kCluster blocks that share a row), of
+// kN = 2 or 4 values at once: the same bits in every thread.  The values part
+// ways on the first exchanges (of four, 16 lanes go on with two each, then 8
+// lanes with one), so four cost six shuffles.  Each warp leaves its sums in the
+// shared memory of every block of the cluster; behind the barrier eight lanes per
+// value add them up.  The two halves of `red` take turns, so a thread that still
+// reads one is never overtaken (the next write to it comes behind the other
+// half's barrier).
+template <int kN, int kW, int kCluster>
+struct GroupSums {
+  static constexpr int kEntries = kW * kCluster;                  // per value
+  static constexpr int kPerLane = (kEntries + 7) / 8;
+  float part[2][kN][8 * kPerLane];
+};
+
+__device__ __forceinline__ void store_in_block(float* p, uint32_t block, float v) {
+  uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p));
+  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(block));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t block_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <int kN, int kW, int kCluster>
+__device__ __forceinline__ void group_all_sum(float (&v)[kN], GroupSums<kN, kW, kCluster>& red, int& parity, int group) {
+  static_assert(kN == 2 || kN == 4, "values");
+  using R = GroupSums<kN, kW, kCluster>;
+  const int lane = threadIdx.x & 31;
+  const bool up = lane & 16;
+  constexpr int kLanes = 32 / kN;  // that go on with one value
+  float a;
+  if constexpr (kN == 4) {
+    const bool right = lane & 8;
+    a = (up ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
+    const float b = (up ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+    a = (right ? b : a) + __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
+  } else {
+    a = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+  }
+#pragma unroll
+  for (int o = kLanes / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  if constexpr (kW * kCluster > 1) {
+    float(*r)[8 * R::kPerLane] = red.part[parity];
+    parity ^= 1;
+    const int warp = (threadIdx.x >> 5) % kW;
+    if constexpr (kCluster == 1) {
+      if (lane % kLanes == 0) r[lane / kLanes][warp] = a;
+      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * kW) : "memory");
+    } else {
+      const int entry = block_in_cluster() * kW + warp;
+      if (lane % kLanes < kCluster) store_in_block(&r[lane / kLanes][entry], lane % kLanes, a);
+      cluster_barrier();
+    }
+    const int at = (lane & 7) * R::kPerLane;
+    const float* mine = r[(lane >> 3) % kN] + at;
+    a = 0.0f;
+#pragma unroll
+    for (int i = 0; i < R::kPerLane; ++i)
+      if (at + i < R::kEntries) a += mine[i];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, kLanes * i);
+  }
+}
+
+// Two rows at a time, 16 elements of each to a thread; the sums of the next two
+// rows and the squared deviations of the current two are reduced together, so
+// two rows cost one barrier and six shuffles although each variance is taken
+// about its row's exact mean.
+template <class T, int kW, int kGroups, int kCluster, int kStages, bool kFull>
+__global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel(const ForwardArgs a) {
+  pdl_entry();
+  using U = Unit<T>;
+  constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
+  using S = Stream<T, kUnits, kW, kGroups, kStages, 2>;
+  extern __shared__ __align__(16) uint4 ring[];
+  __shared__ GroupSums<4, kW, kCluster> red[kGroups];
+  // the thread within the row's threads of all blocks; they are kTpr
+  constexpr int kTpr = S::kTpg * kCluster;
+  const int group = threadIdx.x / S::kTpg;
+  const int t = threadIdx.x % S::kTpg + (kCluster > 1 ? static_cast<int>(block_in_cluster()) * S::kTpg : 0);
+  auto live = [&](int i) { return kFull || (i * kTpr + t) * kPer < a.cols; };
+  uint4* const mine = ring + threadIdx.x;
+  // rows 2 p and 2 p + 1 of pair p = cluster + clusters * (group + kGroups * j)
+  const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
+  const int step = 2 * clusters * kGroups;
+  int row = 2 * (cluster + clusters * group);
+  if constexpr (kCluster > 1) cluster_barrier();  // every block of it runs before one stores into another
+  int ahead_row = row;
+  const T* ahead = static_cast<const T*>(a.x) + ahead_row * a.x_stride + t * kPer;
+  auto fetch = [&](int stage) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (ahead_row + k < a.rows) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i)
+          if (live(i))
+            copy_unit_async(mine + ((stage * 2 + k) * kUnits + i) * S::kThreads, ahead + k * a.x_stride + i * kTpr * kPer);
+      }
+    }
+    copies_commit();
+    ahead += step * a.x_stride;
+    ahead_row += step;
+  };
+  // this thread's units of row r (that has arrived), and their sum
+  auto take = [&](int r, int stage, int k, uint4 (&q)[kUnits]) {
+    F2 s = f2(0.0f);
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      q[i] = r < a.rows && live(i) ? mine[((stage * 2 + k) * kUnits + i) * S::kThreads] : no_unit();
+      F2 v[kPairs];
+      U::pairs(q[i], v);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) s = add2(s, v[j]);
+    }
+    return sum2(s);
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(k);
+  F2 w[kUnits][kPairs], b[kUnits][kPairs];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    load_param_pairs<kPer>(live(i) ? a.weight : nullptr, (i * kTpr + t) * kPer, 1.0f, w[i]);
+    load_param_pairs<kPer>(live(i) ? a.bias : nullptr, (i * kTpr + t) * kPer, 0.0f, b[i]);
+  }
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  int parity = 0, stage = 0;
+  uint4 q[2][kUnits];
+  float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f}, mu[2];
+  copies_wait<kStages - 2>();
+#pragma unroll
+  for (int k = 0; k < 2; ++k) sums[k] = take(row + k, 0, k, q[k]);
+  group_all_sum(sums, red[group], parity, group);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) mu[k] = div_by(sums[k], n, inv_n);
+  T* yr = static_cast<T*>(a.y) + row * a.y_stride + t * kPer;
+  for (; row < a.rows; row += step) {
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    copies_wait<kStages - 2>();
+    uint4 next[2][kUnits];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sums[k] = take(row + step + k, stage, k, next[k]);
+      const F2 minus_mu = f2(-mu[k]);
+      F2 d2 = f2(0.0f);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        F2 v[kPairs];
+        U::pairs(q[k][i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const F2 d = add2(v[j], minus_mu);
+          if (live(i)) d2 = fma2(d, d, d2);
+        }
+      }
+      sums[2 + k] = sum2(d2);
+    }
+    group_all_sum(sums, red[group], parity, group);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (row + k >= a.rows) break;
+      const float r = rsqrtf(div_by(sums[2 + k], n, inv_n) + a.eps);
+      if (t == 0) {
+        if (a.mean) a.mean[row + k] = mu[k];
+        if (a.rstd) a.rstd[row + k] = r;
+      }
+      const F2 rr = f2(r), minus_mu = f2(-mu[k]);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        if (!live(i)) continue;
+        F2 v[kPairs];
+        U::pairs(q[k][i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) v[j] = fma2(mul2(add2(v[j], minus_mu), rr), w[i][j], b[i][j]);
+        U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
+      }
+    }
+    yr += step * a.y_stride;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      mu[k] = div_by(sums[k], n, inv_n);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) q[k][i] = next[k][i];
+    }
+  }
+  copies_wait<0>();
+}
+
+struct BackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const float* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  int64_t dx_stride;
+  float* part;  // [slabs][dw, db][cols], or null: no parameter gradients are wanted
+  int rows, cols;
+};
+
+// dx, and the column sums of each slab (the rows of one cluster), in one read of dy
+// and x: a thread adds up its 16 columns in registers over all its rows, the
+// block's groups are added in shared memory at the end.  kRows rows at a time.
+template <class T, int kW, int kGroups, int kCluster, int kRows, int kStages, bool kFull>
+__global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kernel(const BackwardArgs a) {
+  pdl_entry();
+  using U = Unit<T>;
+  constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
+  using S = Stream<T, kUnits, kW, kGroups, kStages, 2 * kRows>;
+  extern __shared__ __align__(16) uint4 ring[];
+  __shared__ GroupSums<2 * kRows, kW, kCluster> red[kGroups];
+  constexpr int kTpr = S::kTpg * kCluster;
+  const int group = threadIdx.x / S::kTpg;
+  const int t = threadIdx.x % S::kTpg + (kCluster > 1 ? static_cast<int>(block_in_cluster()) * S::kTpg : 0);
+  auto live = [&](int i) { return kFull || (i * kTpr + t) * kPer < a.cols; };
+  uint4* const mine = ring + threadIdx.x;
+  const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
+  const int step = kRows * clusters * kGroups;
+  int row = kRows * (cluster + clusters * group);
+  if constexpr (kCluster > 1) cluster_barrier();  // every block of it runs before one stores into another
+  int ahead_row = row;
+  const T* dy_ahead = static_cast<const T*>(a.dy) + row * a.dy_stride + t * kPer;
+  const T* x_ahead = static_cast<const T*>(a.x) + row * a.x_stride + t * kPer;
+  auto slot = [&](int stage, int k, int operand, int i) {
+    return mine + (((stage * kRows + k) * 2 + operand) * kUnits + i) * S::kThreads;
+  };
+  auto fetch = [&](int stage) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (ahead_row + k < a.rows) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          if (live(i)) {
+            copy_unit_async(slot(stage, k, 0, i), dy_ahead + k * a.dy_stride + i * kTpr * kPer);
+            copy_unit_async(slot(stage, k, 1, i), x_ahead + k * a.x_stride + i * kTpr * kPer);
+          }
+        }
+      }
+    }
+    copies_commit();
+    dy_ahead += step * a.dy_stride;
+    x_ahead += step * a.x_stride;
+    ahead_row += step;
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 1; ++k) fetch(k);
+  F2 w[kUnits][kPairs], dw[kUnits][kPairs], db[kUnits][kPairs];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    load_param_pairs<kPer>(live(i) ? a.weight : nullptr, (i * kTpr + t) * kPer, 1.0f, w[i]);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) dw[i][j] = db[i][j] = f2(0.0f);
+  }
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  int parity = 0, stage = 0;
+  T* dxr = static_cast<T*>(a.dx) + row * a.dx_stride + t * kPer;
+  // the statistics of the rows to come, a step ahead
+  float mu[kRows], r[kRows], next_mu[kRows], next_r[kRows];
+  auto stats = [&](int first, float (&m)[kRows], float (&s)[kRows]) {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      m[k] = first + k < a.rows ? __ldg(a.mean + first + k) : 0.0f;
+      s[k] = first + k < a.rows ? __ldg(a.rstd + first + k) : 0.0f;
+    }
+  };
+  stats(row, mu, r);
+  for (; row < a.rows; row += step) {
+    fetch(stage == 0 ? kStages - 1 : stage - 1);
+    stats(row + step, next_mu, next_r);
+    copies_wait<kStages - 1>();
+    uint4 dyq[kRows][kUnits], xq[kRows][kUnits];
+    float sums[2 * kRows];
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      const F2 minus_mu = f2(-mu[k]), rr = f2(r[k]);
+      F2 s1 = f2(0.0f), s2 = f2(0.0f);
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const bool there = row + k < a.rows && live(i);
+        dyq[k][i] = there ? *slot(stage, k, 0, i) : no_unit();
+        xq[k][i] = there ? *slot(stage, k, 1, i) : no_unit();
+        F2 d[kPairs], v[kPairs];
+        U::pairs(dyq[k][i], d);
+        U::pairs(xq[k][i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const F2 xh = mul2(add2(v[j], minus_mu), rr), g = mul2(d[j], w[i][j]);
+          db[i][j] = add2(db[i][j], d[j]);
+          dw[i][j] = fma2(d[j], xh, dw[i][j]);
+          s1 = add2(s1, g);
+          s2 = fma2(g, xh, s2);
+        }
+      }
+      sums[2 * k] = sum2(s1);
+      sums[2 * k + 1] = sum2(s2);
+    }
+    stage = stage + 1 == kStages ? 0 : stage + 1;
+    group_all_sum(sums, red[group], parity, group);
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (row + k >= a.rows) break;
+      const F2 minus_mu = f2(-mu[k]), rr = f2(r[k]);
+      const F2 minus_c1 = f2(-div_by(sums[2 * k], n, inv_n)), minus_c2 = f2(-div_by(sums[2 * k + 1], n, inv_n));
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        if (!live(i)) continue;
+        F2 d[kPairs], v[kPairs];
+        U::pairs(dyq[k][i], d);
+        U::pairs(xq[k][i], v);
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          const F2 xh = mul2(add2(v[j], minus_mu), rr);
+          v[j] = mul2(fma2(xh, minus_c2, fma2(d[j], w[i][j], minus_c1)), rr);
+        }
+        U::store_pairs(dxr + k * a.dx_stride + i * kTpr * kPer, v);
+      }
+    }
+    dxr += step * a.dx_stride;
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      mu[k] = next_mu[k];
+      r[k] = next_r[k];
+    }
+  }
+  copies_wait<0>();
+  if (!a.part) return;
+  // the groups' column sums, added in group order
+  if constexpr (kGroups > 1) {
+    __syncthreads();
+    F2* const cell = reinterpret_cast<F2*>(ring);  // [group - 1][dw, db][unit][pair][thread]
+    static_assert(2 * kUnits * kPairs * 8 <= static_cast<int>(S::kSmem / S::kThreads), "the ring holds the groups' sums");
+    auto at = [&](int g, int which, int i, int j) {
+      return cell + ((((g - 1) * 2 + which) * kUnits + i) * kPairs + j) * S::kTpg + threadIdx.x % S::kTpg;
+    };
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          *at(group, 0, i, j) = dw[i][j];
+          *at(group, 1, i, j) = db[i][j];
+        }
+      }
+    }
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < kGroups; ++g) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+#pragma unroll
+        for (int j = 0; j < kPairs; ++j) {
+          dw[i][j] = add2(dw[i][j], *at(g, 0, i, j));
+          db[i][j] = add2(db[i][j], *at(g, 1, i, j));
+        }
+      }
+    }
+  }
+  float* const out = a.part + static_cast<int64_t>(cluster) * 2 * a.cols + t * kPer;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (!live(i)) continue;
+#pragma unroll
+    for (int j = 0; j < kPairs; j += 2) {
+      const float2 a0 = split(dw[i][j]), a1 = split(dw[i][j + 1]), b0 = split(db[i][j]), b1 = split(db[i][j + 1]);
+      *reinterpret_cast<float4*>(out + i * kTpr * kPer + 2 * j) = make_float4(a0.x, a0.y, a1.x, a1.y);
+      *reinterpret_cast<float4*>(out + a.cols + i * kTpr * kPer + 2 * j) = make_float4(b0.x, b0.y, b1.x, b1.y);
+    }
+  }
+}
+
+// Rows of any length: one block per row, three reads of it.
 template <class T>
 __global__ void __launch_bounds__(kThreads)
     layer_norm_row_kernel(const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight,
@@ -97,50 +741,230 @@ __global__ void __launch_bounds__(kThreads)
   part[(2 * static_cast<int64_t>(blockIdx.y) + 1) * cols + c] = db;
 }
 
-// dw and db from the slabs' partial sums, in slab order; zeros for no slab.
+// dw and db from the slabs' partial sums [slabs][2 cols]; zeros for no slab.  A block
+// folds 32 columns: warp w adds slabs w, w + kWarps, ... in order, then the warps are
+// added in order.
 __global__ void __launch_bounds__(kThreads)
     layer_norm_fold_kernel(const float* __restrict__ part, int slabs, float* __restrict__ dweight,
-                           float* __restrict__ dbias, int64_t cols) {
+                           float* __restrict__ dbias, int cols) {
   pdl_entry();
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x;
-  if (c >= cols) return;
-  float dw = 0.0f, db = 0.0f;
-  for (int s = 0; s < slabs; ++s) {
-    dw += part[(2 * static_cast<int64_t>(s)) * cols + c];
-    db += part[(2 * static_cast<int64_t>(s) + 1) * cols + c];
+  __shared__ float red[kWarps][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of 2 cols
+  float s = 0.0f;
+  if (c < 2 * static_cast<int64_t>(cols)) {
+#pragma unroll 4
+    for (int k = warp; k < slabs; k += kWarps) s += part[k * 2 * static_cast<int64_t>(cols) + c];
   }
-  if (dweight) dweight[c] = dw;
-  if (dbias) dbias[c] = db;
+  red[warp][lane] = s;
+  __syncthreads();
+  if (warp > 0 || c >= 2 * static_cast<int64_t>(cols)) return;
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) s += red[w][lane];
+  if (c < cols) {
+    if (dweight) dweight[c] = s;
+  } else if (dbias) {
+    dbias[c - cols] = s;
+  }
 }
+
+// Whether every row of these tensors is a whole number of 16-byte units from a
+// 16-byte boundary on.
+bool whole_units(std::initializer_list<const void*> tensors, std::initializer_list<int64_t> strides, int64_t rows,
+                 int64_t cols, std::size_t elem) {
+  const int64_t per = 16 / static_cast<int64_t>(elem);
+  bool ok = cols % per == 0;
+  for (const void* p : tensors) ok = ok && aligned(p, 16);
+  for (int64_t st : strides) ok = ok && (rows <= 1 || st % per == 0);
+  return ok;
+}
+
+// Rows up to which a launch is bound by one row's latency, not by bandwidth: a
+// row is then spread over as many threads as it has units.
+constexpr int64_t kFewRows = 4 * 148;
+
+// One persistent block on each SM of a B200, a constant so that results do not
+// depend on the device.
+constexpr int64_t kStreamBlocks = 148;
 
 // Slabs of rows whose column sums are kept apart.  From the extents alone, so
 // the order of the sums, and every bit of dw and db, is the same on any GPU.
 int64_t column_slabs(int64_t rows) { return rows < 148 ? rows : 148; }
 
-template <class T>
-void launch_forward(const void* x, int64_t x_stride, const float* weight, const float* bias, void* y, int64_t y_stride,
-                    float* mean, float* rstd, int64_t rows, int64_t cols, float eps, cudaStream_t s) {
-  launch_async(layer_norm_row_kernel<T>, static_cast<unsigned>(rows), kThreads, 0, s, static_cast<const T*>(x),
-               x_stride, weight, bias, static_cast<T*>(y), y_stride, mean, rstd, cols, eps);
+// Calls f with the smallest of the unit counts kUnits, 2 kUnits .. kMax that holds n
+// units over `threads` threads, and with whether they are filled.
+template <int kMax, int kUnits = 1, class F>
+void with_units(int64_t n, int64_t threads, F&& f) {
+  if constexpr (kUnits < kMax) {
+    if (n > kUnits * threads) return with_units<kMax, 2 * kUnits>(n, threads, f);
+  }
+  if (n == kUnits * threads) f(std::integral_constant<int, kUnits>{}, std::true_type{});
+  else f(std::integral_constant<int, kUnits>{}, std::false_type{});
+}
+// Calls f with n, of 1 .. kMax.
+template <int kMax, int kN = 1, class F>
+void with_count(int64_t n, F&& f) {
+  if constexpr (kN < kMax) {
+    if (n > kN) return with_count<kMax, kN + 1>(n, f);
+  }
+  f(std::integral_constant<int, kN>{});
+}
+
+// Launches a persistent kernel of one block per SM, in clusters of kCluster: as many
+// clusters as there are items, kStreamBlocks blocks at most.  Returns the clusters.
+template <int kCluster, class A>
+int64_t launch_stream(void (*kernel)(const A), const A& a, int64_t items, int threads, std::size_t smem, cudaStream_t s) {
+  // the attribute is a property of the kernel on the current device: set it every time
+  cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       static_cast<int>(smem));
+  const int64_t clusters = items < kStreamBlocks / kCluster ? items : kStreamBlocks / kCluster;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  if (kCluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = kCluster;
+    attr[cfg.numAttrs].val.clusterDim.y = 1;
+    attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (pdl_enabled()) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  cudaLaunchKernelEx(&cfg, kernel, a);  // errors are left for check_launch()
+  return clusters;
+}
+
+// Calls f(warps, blocks) with the smallest group, of 1 .. 16 warps in each of 1, 2 or 4
+// blocks, whose threads hold a row of `cols` <= kStreamCols at 16 elements each.
+constexpr int64_t kStreamCols = 4 * 8192;
+template <class F>
+void with_group(int64_t cols, F&& f) {
+  using std::integral_constant;
+  const int64_t warps = (cols + 511) / 512;
+  const integral_constant<int, 1> one;
+  if (warps <= 1) f(one, one);
+  else if (warps <= 2) f(integral_constant<int, 2>{}, one);
+  else if (warps <= 3) f(integral_constant<int, 3>{}, one);
+  else if (warps <= 4) f(integral_constant<int, 4>{}, one);
+  else if (warps <= 6) f(integral_constant<int, 6>{}, one);
+  else if (warps <= 8) f(integral_constant<int, 8>{}, one);
+  else if (warps <= 12) f(integral_constant<int, 12>{}, one);
+  else if (warps <= 16) f(integral_constant<int, 16>{}, one);
+  else if (warps <= 24) f(integral_constant<int, 12>{}, integral_constant<int, 2>{});
+  else if (warps <= 32) f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  else if (warps <= 48) f(integral_constant<int, 12>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
 }
 
 template <class T>
-void launch_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, const float* weight,
-                     const float* mean, const float* rstd, void* dx, int64_t dx_stride, float* dweight, float* dbias,
-                     int64_t rows, int64_t cols, float* part, cudaStream_t s) {
-  const T* dyt = static_cast<const T*>(dy);
-  const T* xt = static_cast<const T*>(x);
-  const unsigned blocks = static_cast<unsigned>((cols + kThreads - 1) / kThreads);
-  const int64_t slabs = column_slabs(rows);
-  if (rows > 0)
-    launch_async(layer_norm_dx_kernel<T>, static_cast<unsigned>(rows), kThreads, 0, s, dyt, dy_stride, xt, x_stride,
-                 weight, mean, rstd, static_cast<T*>(dx), dx_stride, cols);
-  if (!dweight && !dbias) return;
-  if (rows > 0)
-    launch_async(layer_norm_columns_kernel<T>, dim3(blocks, static_cast<unsigned>(slabs)), kThreads, 0, s, dyt,
-                 dy_stride, xt, x_stride, mean, rstd, part, rows, cols);
-  launch_async(layer_norm_fold_kernel, blocks, kThreads, 0, s, static_cast<const float*>(part),
-               static_cast<int>(slabs), dweight, dbias, cols);
+void launch_forward_stream(const ForwardArgs& a, cudaStream_t s) {
+  constexpr int kStages = 3;
+  with_group(a.cols, [&](auto warps, auto blocks) {
+    constexpr int kW = decltype(warps)::value, kC = decltype(blocks)::value;
+    constexpr int kGroups = kW == 1 ? 15 : 16 / kW;
+    using S = Stream<T, 16 / Unit<T>::kPer, kW, kGroups, kStages, 2>;
+    const int64_t pairs = (a.rows + 1) / 2;
+    if (a.cols == 512 * kW * kC)
+      launch_stream<kC>(layer_norm_stream_kernel<T, kW, kGroups, kC, kStages, true>, a, pairs, S::kThreads, S::kSmem, s);
+    else
+      launch_stream<kC>(layer_norm_stream_kernel<T, kW, kGroups, kC, kStages, false>, a, pairs, S::kThreads, S::kSmem, s);
+  });
+}
+
+template <class T>
+void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
+  using std::integral_constant;
+  constexpr int kPer = Unit<T>::kPer;
+  const unsigned rows = static_cast<unsigned>(a.rows);
+  const bool few = a.rows <= kFewRows;
+  const int64_t n = a.cols / kPer;  // units
+  // a row's kW warps hold it at up to kMax units a thread
+  auto row_kernel = [&](auto w, auto max) {
+    constexpr int kW = decltype(w)::value;
+    with_units<decltype(max)::value>(n, 32 * kW, [&](auto units, auto full) {
+      launch_async(layer_norm_kernel<T, decltype(units)::value, kW, decltype(full)::value>,
+                   kW == 1 ? (rows + kWarps - 1) / kWarps : rows, kW == 1 ? kThreads : 32 * kW, 0, s, a);
+    });
+  };
+  auto elements = [&](auto thr, auto max) {
+    constexpr int kThr = decltype(thr)::value;
+    with_count<decltype(max)::value>((a.cols + 2 * kThr - 1) / (2 * kThr), [&](auto pairs) {
+      launch_async(layer_norm_elements_kernel<T, decltype(pairs)::value, kThr>, rows, kThr, 0, s, a);
+    });
+  };
+  if (!whole && a.cols <= (few ? 512 : 4096)) {
+    elements(integral_constant<int, 128>{}, integral_constant<int, 16>{});
+  } else if (!whole && a.cols <= 16384) {
+    elements(integral_constant<int, 512>{}, integral_constant<int, 16>{});
+  } else if (whole && few && n <= 32) {
+    row_kernel(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+  } else if (whole && few && n <= 128) {
+    row_kernel(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+  } else if (whole && !few && (sizeof(T) == 2 || n > 2048) && a.cols <= kStreamCols) {
+    launch_forward_stream<T>(a, s);
+  } else if (whole && sizeof(T) == 4 && !few && n <= 512) {
+    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+  } else if (whole && sizeof(T) == 4 && !few && n <= 1024) {
+    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 2>{}, integral_constant<int, 16>{});
+  } else if (whole && sizeof(T) == 4 && !few && n <= 2048) {
+    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 4>{}, integral_constant<int, 16>{});
+  } else if (whole && n <= 4096) {
+    row_kernel(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+  } else {
+    launch_async(layer_norm_row_kernel<T>, rows, kThreads, 0, s, static_cast<const T*>(a.x), a.x_stride, a.weight,
+                 a.bias, static_cast<T*>(a.y), a.y_stride, a.mean, a.rstd, static_cast<int64_t>(a.cols), a.eps);
+  }
+}
+
+// Returns the number of slabs of partial sums that were written.
+template <class T>
+int64_t launch_backward_stream(const BackwardArgs& a, cudaStream_t s) {
+  // f32 rows take twice the ring: one at a time
+  constexpr int kRows = sizeof(T) == 2 ? 2 : 1, kStages = 3;
+  int64_t slabs = 0;
+  with_group(a.cols, [&](auto warps, auto blocks) {
+    constexpr int kW = decltype(warps)::value, kC = decltype(blocks)::value;
+    constexpr int kGroups = kW == 1 ? 15 : 16 / kW;
+    using S = Stream<T, 16 / Unit<T>::kPer, kW, kGroups, kStages, 2 * kRows>;
+    const int64_t items = (a.rows + kRows - 1) / kRows;
+    if (a.cols == 512 * kW * kC)
+      slabs = launch_stream<kC>(layer_norm_backward_kernel<T, kW, kGroups, kC, kRows, kStages, true>, a, items,
+                                S::kThreads, S::kSmem, s);
+    else
+      slabs = launch_stream<kC>(layer_norm_backward_kernel<T, kW, kGroups, kC, kRows, kStages, false>, a, items,
+                                S::kThreads, S::kSmem, s);
+  });
+  return slabs;
+}
+
+template <class T>
+void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* dbias, cudaStream_t s) {
+  const T* dy = static_cast<const T*>(a.dy);
+  const T* x = static_cast<const T*>(a.x);
+  int64_t slabs = 0;
+  if (a.rows > 0 && whole && a.cols <= kStreamCols) {
+    slabs = launch_backward_stream<T>(a, s);
+  } else if (a.rows > 0) {
+    launch_async(layer_norm_dx_kernel<T>, static_cast<unsigned>(a.rows), kThreads, 0, s, dy, a.dy_stride, x, a.x_stride,
+                 a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.dx_stride, static_cast<int64_t>(a.cols));
+    if (a.part) {
+      slabs = column_slabs(a.rows);
+      launch_async(layer_norm_columns_kernel<T>,
+                   dim3(static_cast<unsigned>((a.cols + kThreads - 1) / kThreads), static_cast<unsigned>(slabs)),
+                   kThreads, 0, s, dy, a.dy_stride, x, a.x_stride, a.mean, a.rstd, a.part, static_cast<int64_t>(a.rows),
+                   static_cast<int64_t>(a.cols));
+    }
+  }
+  if (dweight || dbias)
+    launch_async(layer_norm_fold_kernel, static_cast<unsigned>((2 * static_cast<int64_t>(a.cols) + 31) / 32), kThreads,
+                 0, s, static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
 }
 
 }  // namespace
@@ -170,10 +994,11 @@ extern "C" int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const floa
                          span_of("bias", bias, cols * 4)};
   MCKE_RETURN_IF(check_overlaps(who, outs, ins));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (dtype == MCKE_DTYPE_BF16)
-    launch_forward<uint16_t>(x, x_stride, weight, bias, y, y_stride, mean, rstd, rows, cols, eps, s);
-  else
-    launch_forward<float>(x, x_stride, weight, bias, y, y_stride, mean, rstd, rows, cols, eps, s);
+  const ForwardArgs a = {x, x_stride, weight, bias, y, y_stride, mean, rstd, static_cast<int>(rows),
+                         static_cast<int>(cols), eps};
+  const bool whole = whole_units({x, y}, {x_stride, y_stride}, rows, cols, e) && aligned(weight, 16) && aligned(bias, 16);
+  if (dtype == MCKE_DTYPE_BF16) launch_forward<uint16_t>(a, whole, s);
+  else launch_forward<float>(a, whole, s);
   return check_launch(who);
 }
 
@@ -216,12 +1041,11 @@ extern "C" int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride,
                          span_of("rstd", rstd, rows * 4)};
   MCKE_RETURN_IF(check_overlaps(who, outs, ins));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  float* part = static_cast<float*>(workspace);
-  if (dtype == MCKE_DTYPE_BF16)
-    launch_backward<uint16_t>(dy, dy_stride, x, x_stride, weight, mean, rstd, dx, dx_stride, dweight, dbias, rows,
-                              cols, part, s);
-  else
-    launch_backward<float>(dy, dy_stride, x, x_stride, weight, mean, rstd, dx, dx_stride, dweight, dbias, rows, cols,
-                           part, s);
+  const BackwardArgs a = {dy, dy_stride, x, x_stride, weight, mean, rstd, dx, dx_stride,
+                          params ? static_cast<float*>(workspace) : nullptr, static_cast<int>(rows),
+                          static_cast<int>(cols)};
+  const bool whole = whole_units({dy, x, dx}, {dy_stride, x_stride, dx_stride}, rows, cols, e) && aligned(weight, 16);
+  if (dtype == MCKE_DTYPE_BF16) launch_backward<uint16_t>(a, whole, dweight, dbias, s);
+  else launch_backward<float>(a, whole, dweight, dbias, s);
   return check_launch(who);
 }

@@ -81,6 +81,49 @@ __device__ __forceinline__ float ld_val(const uint16_t* p) { return from_bf16(*p
 __device__ __forceinline__ void st_val(float* p, float v) { *p = v; }
 __device__ __forceinline__ void st_val(uint16_t* p, float v) { *p = to_bf16(v); }
 
+// Two floats in a 64-bit register: one instruction adds, multiplies or fuses both
+// (sm_100's f32x2 forms; each half rounds as its scalar form does).
+struct F2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float both) { return f2(both, both); }
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum2(F2 a) {
+  const float2 s = split(a);
+  return s.x + s.y;
+}
+
+// s / n for a row length n whose reciprocal is at hand: the product, and
+// Markstein's correction of it by the remainder.
+__device__ __forceinline__ float div_by(float s, float n, float inv_n) {
+  const float q = s * inv_n;
+  return fmaf(fmaf(-q, n, s), inv_n, q);
+}
+
 // ---- device: sums --------------------------------------------------------------------
 
 template <class V>

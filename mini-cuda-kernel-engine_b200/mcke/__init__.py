@@ -9,6 +9,7 @@ library is missing the first call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -514,8 +515,9 @@ def _rows_of(t: torch.Tensor, name: str, dtype=None) -> tuple[int, int, int]:
         raise ValueError(f"{name} must be {dtype or 'float32 or bfloat16'}, got {t.dtype}")
     if t.dim() == 2:
         rows, cols = t.shape
-        if t.stride(1) == 1 or cols <= 1:
-            return rows, cols, t.stride(0)
+        stride, inner = t.stride()
+        if inner == 1 or cols <= 1:
+            return rows, cols, stride
     elif t.dim() > 0 and t.is_contiguous():
         cols = t.shape[-1]
         return (t.numel() // cols if cols else math.prod(t.shape[:-1])), cols, cols
@@ -526,7 +528,7 @@ def _vector(t, n: int, dtype, name: str, like: torch.Tensor) -> int | None:
     """Address of a contiguous vector of n elements on like's device (None stays None)."""
     if t is None:
         return None
-    if t.device != like.device:
+    if t.get_device() != like.get_device():
         raise ValueError(f"{name} must be on {like.device}, got {t.device}")
     if t.dtype != dtype or t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be {n} contiguous values of {dtype}, got {tuple(t.shape)} of {t.dtype}")
@@ -539,53 +541,52 @@ def _same(t, like: torch.Tensor, name: str) -> None:
                          f"{t.device}")
 
 
-class _On:
-    """The device and stream of one call: current inside the ``with``, so that
-    launches reach them and allocations belong to them.  Nothing is switched
-    where both are current already."""
-    __slots__ = ("handle", "_guards")
+def _elsewhere(t: torch.Tensor, stream) -> bool:
+    """Whether a call has to switch to t's device or to ``stream`` first."""
+    return stream is not None or torch.cuda.current_device() != t.get_device()
 
-    def __init__(self, device: torch.device, stream):
-        self._guards = []
-        if torch.cuda.current_device() != device.index:
-            self._guards.append(torch.cuda.device(device))
-        self.handle = torch.cuda.current_stream(device).cuda_stream
-        if stream is not None:
-            handle = stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
-            if handle != self.handle:
-                if not hasattr(stream, "cuda_stream"):
-                    stream = torch.cuda.ExternalStream(handle, device=device)
-                self._guards.append(torch.cuda.stream(stream))
-                self.handle = handle
 
-    def __enter__(self) -> int:
-        for g in self._guards:
-            g.__enter__()
-        return self.handle
+@contextlib.contextmanager
+def _on(t: torch.Tensor, stream):
+    """t's device, and ``stream`` (a torch stream, or a raw handle), made current: launches
+    reach them and allocations belong to them."""
+    with torch.cuda.device(t.device):
+        if stream is None:
+            yield
+            return
+        if not hasattr(stream, "cuda_stream"):
+            handle = int(stream)
+            stream = (torch.cuda.ExternalStream(handle, device=t.device) if handle
+                      else torch.cuda.default_stream(t.device))
+        with torch.cuda.stream(stream):
+            yield
 
-    def __exit__(self, *exc):
-        for g in reversed(self._guards):
-            g.__exit__(*exc)
+
+def _current(t: torch.Tensor) -> int:
+    """Handle of the current stream of t's device."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, out=None, save_stats: bool = False, stream=None):
     """Layer norm over the last dimension (mcke_sm100_layer_norm): x float32 or
     bfloat16, weight and bias float32 [cols] or None.  Returns y, or (y, mean,
-    rstd) with ``save_stats``: the float32 row statistics that
+    rstd) with ``save_stats``: the float32 statistics, one per row, that
     :func:`layer_norm_backward` takes."""
     rows, cols, xs = _rows_of(x, "x")
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return layer_norm(x, weight, bias, eps, out, save_stats)
     w, b = _vector(weight, cols, torch.float32, "weight", x), _vector(bias, cols, torch.float32, "bias", x)
-    if out is not None:
+    if out is None:
+        out, ys = torch.empty_like(x, memory_format=torch.contiguous_format), cols
+    else:
         _same(out, x, "out")
         ys = _rows_of(out, "out", x.dtype)[2]
-    with _On(x.device, stream) as s:
-        if out is None:
-            out, ys = torch.empty(x.shape, dtype=x.dtype, device=x.device), cols
-        mean = rstd = None
-        if save_stats:
-            mean, rstd = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        _check(lib().mcke_sm100_layer_norm(x.data_ptr(), xs, w, b, out.data_ptr(), ys, _ptr(mean), _ptr(rstd), rows,
-                                           cols, eps, _DTYPE_OF[x.dtype], s))
+    mean = rstd = None
+    if save_stats:
+        mean, rstd = x.new_empty(rows, dtype=torch.float32), x.new_empty(rows, dtype=torch.float32)
+    _check(lib().mcke_sm100_layer_norm(x.data_ptr(), xs, w, b, out.data_ptr(), ys, _ptr(mean), _ptr(rstd), rows, cols,
+                                       eps, _DTYPE_OF[x.dtype], _current(x)))
     return (out, mean, rstd) if save_stats else out
 
 
@@ -599,27 +600,28 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None, param_grads: b
     dweight, dbias), dx in x's type, the others float32 [cols]; only dx without
     ``param_grads``."""
     rows, cols, xs = _rows_of(x, "x")
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return layer_norm_backward(dy, x, mean, rstd, weight, out, param_grads, workspace)
     _same(dy, x, "dy")
     dys = _rows_of(dy, "dy", x.dtype)[2]
     m, r = _vector(mean, rows, torch.float32, "mean", x), _vector(rstd, rows, torch.float32, "rstd", x)
     w = _vector(weight, cols, torch.float32, "weight", x)
-    if out is not None:
+    if out is None:
+        out, dxs = torch.empty_like(x, memory_format=torch.contiguous_format), cols
+    else:
         _same(out, x, "out")
         dxs = _rows_of(out, "out", x.dtype)[2]
+    dw = db = None
+    if param_grads:
+        dw, db = x.new_empty(cols, dtype=torch.float32), x.new_empty(cols, dtype=torch.float32)
+        if workspace is None:
+            workspace = x.new_empty(layer_norm_backward_workspace_bytes(rows, cols), dtype=torch.uint8)
     if workspace is not None and workspace.device != x.device:
         raise ValueError(f"workspace must be on {x.device}")
-    with _On(x.device, stream) as s:
-        if out is None:
-            out, dxs = torch.empty(x.shape, dtype=x.dtype, device=x.device), cols
-        dw = db = None
-        if param_grads:
-            dw, db = torch.empty((2, cols), dtype=torch.float32, device=x.device)
-            if workspace is None:
-                workspace = torch.empty(layer_norm_backward_workspace_bytes(rows, cols), dtype=torch.uint8,
-                                        device=x.device)
-        _check(lib().mcke_sm100_layer_norm_backward(
-            dy.data_ptr(), dys, x.data_ptr(), xs, w, m, r, out.data_ptr(), dxs, _ptr(dw), _ptr(db), rows, cols,
-            _DTYPE_OF[x.dtype], _ptr(workspace), 0 if workspace is None else workspace.nbytes, s))
+    _check(lib().mcke_sm100_layer_norm_backward(
+        dy.data_ptr(), dys, x.data_ptr(), xs, w, m, r, out.data_ptr(), dxs, _ptr(dw), _ptr(db), rows, cols,
+        _DTYPE_OF[x.dtype], _ptr(workspace), 0 if workspace is None else workspace.nbytes, _current(x)))
     return (out, dw, db) if param_grads else out
 
 
@@ -641,19 +643,21 @@ def token_logprobs(logits, targets=None, top_k: int = 0, entropy: bool = False, 
     entropy, and the ``top_k`` likeliest tokens (log probabilities and int64 ids).
     Shapes are logits' without the last dimension (and [..., top_k])."""
     rows, cols, xs = _rows_of(logits, "logits")
+    if _elsewhere(logits, stream):
+        with _on(logits, stream):
+            return token_logprobs(logits, targets, top_k, entropy)
     t = _vector(targets, rows, torch.int64, "targets", logits)
-    shape, dev = logits.shape[:-1], logits.device
-    with _On(dev, stream) as s:
-        n = 1 + (targets is not None) + bool(entropy)
-        vals = torch.empty((n, *shape), dtype=torch.float32, device=dev).unbind(0)
-        lse, lp, ent = vals[0], vals[1] if targets is not None else None, vals[-1] if entropy else None
-        top = ids = None
-        if top_k:
-            k = max(int(top_k), 0)  # the library refuses a negative one
-            top = torch.empty((*shape, k), dtype=torch.float32, device=dev)
-            ids = torch.empty((*shape, k), dtype=torch.int64, device=dev)
-        _check(lib().mcke_sm100_token_logprobs(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype], t, _ptr(lp),
-                                               lse.data_ptr(), _ptr(ent), top_k, _ptr(top), _ptr(ids), s))
+    shape = logits.shape[:-1]
+    lse = logits.new_empty(shape, dtype=torch.float32)
+    lp = None if targets is None else logits.new_empty(shape, dtype=torch.float32)
+    ent = logits.new_empty(shape, dtype=torch.float32) if entropy else None
+    top = ids = None
+    if top_k:
+        k = max(int(top_k), 0)  # the library refuses a negative one
+        top = logits.new_empty((*shape, k), dtype=torch.float32)
+        ids = logits.new_empty((*shape, k), dtype=torch.int64)
+    _check(lib().mcke_sm100_token_logprobs(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype], t, _ptr(lp),
+                                           lse.data_ptr(), _ptr(ent), top_k, _ptr(top), _ptr(ids), _current(logits)))
     return TokenLogprobs(lp, lse, ent, top, ids)
 
 
@@ -663,17 +667,19 @@ def token_logprobs_backward(logits, lse, targets=None, grad_logprobs=None, entro
     entropy and lse (mcke_sm100_token_logprobs_backward), in logits' type.
     ``out`` may be ``logits`` itself."""
     rows, cols, xs = _rows_of(logits, "logits")
+    if _elsewhere(logits, stream):
+        with _on(logits, stream):
+            return token_logprobs_backward(logits, lse, targets, grad_logprobs, entropy, grad_entropy, grad_lse, out)
     f = lambda v, name: _vector(v, rows, torch.float32, name, logits)  # noqa: E731
     args = (f(lse, "lse"), _vector(targets, rows, torch.int64, "targets", logits), f(grad_logprobs, "grad_logprobs"),
             f(entropy, "entropy"), f(grad_entropy, "grad_entropy"), f(grad_lse, "grad_lse"))
-    if out is not None:
+    if out is None:
+        out, ds = torch.empty_like(logits, memory_format=torch.contiguous_format), cols
+    else:
         _same(out, logits, "out")
         ds = _rows_of(out, "out", logits.dtype)[2]
-    with _On(logits.device, stream) as s:
-        if out is None:
-            out, ds = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device), cols
-        _check(lib().mcke_sm100_token_logprobs_backward(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype],
-                                                        *args, out.data_ptr(), ds, s))
+    _check(lib().mcke_sm100_token_logprobs_backward(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype], *args,
+                                                    out.data_ptr(), ds, _current(logits)))
     return out
 
 
@@ -683,38 +689,47 @@ class Grad(ctypes.Structure):
                 ("dtype", ctypes.c_int), ("out_dtype", ctypes.c_int)]
 
 
-def _grad_list(grads, outs):
-    """(mcke_grad array, count, device) of contiguous float32 and bfloat16 tensors."""
+_GRAD_FORMAT = "QQqii"  # Grad's fields for struct.pack: a tenth of the time of filling them one by one
+
+
+def _grad_list(grads, outs) -> bytes:
+    """The mcke_grad array of contiguous float32 and bfloat16 tensors of one device."""
     if not grads:
         raise ValueError("the list of gradients is empty")
     if len(outs) != len(grads):
         raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
-    dev = grads[0].device
-    for kind, tensors in (("gradient", grads), ("output", outs)):
+    index, fields = grads[0].get_device(), []
+    for kind, tensors in (("gradient", grads),) if outs is grads else (("gradient", grads), ("output", outs)):
         for i, t in enumerate(tensors):
-            if not t.is_cuda or t.device != dev or t.dtype not in _DTYPE_OF or not t.is_contiguous():
+            if index < 0 or t.get_device() != index or t.dtype not in _DTYPE_OF or not t.is_contiguous():
                 raise ValueError(f"{kind} {i} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
-    if outs is not grads:
+    if outs is grads:
+        for g in grads:
+            p, d = g.data_ptr(), _DTYPE_OF[g.dtype]
+            fields += (p, p, g.numel(), d, d)
+    else:
         for i, (g, o) in enumerate(zip(grads, outs)):
             if g.shape != o.shape:
                 raise ValueError(f"output {i} must have shape {tuple(g.shape)}, got {tuple(o.shape)}")
-    arr = (Grad * len(grads))(*[(g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE_OF[g.dtype], _DTYPE_OF[o.dtype])
-                                for g, o in zip(grads, outs)])
-    return arr, len(grads), dev
+            fields += (g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE_OF[g.dtype], _DTYPE_OF[o.dtype])
+    return struct.pack(_GRAD_FORMAT * len(grads), *fields)
 
 
-def _norm_call(arr, n, dev, stream, norm, workspace, call):
-    with _On(dev, stream) as s:
-        if norm is None:
-            norm = torch.empty((), dtype=torch.float32, device=dev)
-        elif norm.device != dev or norm.dtype != torch.float32 or norm.numel() != 1:
-            raise ValueError(f"norm must be one float32 on {dev}")
-        if workspace is None:
-            workspace = torch.empty(grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-        elif workspace.device != dev:
-            raise ValueError(f"workspace must be on {dev}")
-        _check(call(norm.data_ptr(), workspace.data_ptr(), workspace.nbytes, s))
-    return norm
+def _one_float(norm, like) -> None:
+    if norm.device != like.device or norm.dtype != torch.float32 or norm.numel() != 1:
+        raise ValueError(f"norm must be one float32 on {like.device}")
+
+
+def _norm_buffers(grads, norm, workspace):
+    if norm is None:
+        norm = grads[0].new_empty((), dtype=torch.float32)
+    else:
+        _one_float(norm, grads[0])
+    if workspace is None:
+        workspace = grads[0].new_empty(grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8)
+    elif workspace.device != grads[0].device:
+        raise ValueError(f"workspace must be on {grads[0].device}")
+    return norm, workspace
 
 
 def grad_norm_workspace_bytes(count: int) -> int:
@@ -724,29 +739,40 @@ def grad_norm_workspace_bytes(count: int) -> int:
 def grad_norm(grads, norm=None, workspace=None, stream=None):
     """The L2 norm over every element of a list of contiguous float32 and bfloat16
     tensors (mcke_sm100_grad_norm): one float32 on their device."""
-    arr, n, dev = _grad_list(grads, grads)
-    return _norm_call(arr, n, dev, stream, norm, workspace,
-                      lambda *a: lib().mcke_sm100_grad_norm(arr, n, *a))
+    arr = _grad_list(grads, grads)
+    if _elsewhere(grads[0], stream):
+        with _on(grads[0], stream):
+            return grad_norm(grads, norm, workspace)
+    norm, workspace = _norm_buffers(grads, norm, workspace)
+    _check(lib().mcke_sm100_grad_norm(arr, len(grads), norm.data_ptr(), workspace.data_ptr(), workspace.nbytes,
+                                      _current(norm)))
+    return norm
 
 
 def clip_grad_norm(grads, max_norm: float, out=None, norm=None, workspace=None, stream=None):
     """Scales the gradients by min(1, max_norm / (norm + 1e-6))
     (mcke_sm100_clip_grad_norm), in place or into the tensors of ``out`` (the
     gradients' types, or float32).  Returns the norm before clipping."""
-    arr, n, dev = _grad_list(grads, grads if out is None else out)
-    return _norm_call(arr, n, dev, stream, norm, workspace,
-                      lambda *a: lib().mcke_sm100_clip_grad_norm(arr, n, max_norm, *a))
+    arr = _grad_list(grads, grads if out is None else out)
+    if _elsewhere(grads[0], stream):
+        with _on(grads[0], stream):
+            return clip_grad_norm(grads, max_norm, out, norm, workspace)
+    norm, workspace = _norm_buffers(grads, norm, workspace)
+    _check(lib().mcke_sm100_clip_grad_norm(arr, len(grads), max_norm, norm.data_ptr(), workspace.data_ptr(),
+                                           workspace.nbytes, _current(norm)))
+    return norm
 
 
 def clip_grads(grads, max_norm: float, norm, out=None, stream=None) -> None:
     """:func:`clip_grad_norm` by a norm that the caller has on the device
     (mcke_sm100_clip_grads): that of all ranks' gradients, for instance, which
     is the root of the sum of the ranks' squared norms."""
-    arr, n, dev = _grad_list(grads, grads if out is None else out)
-    if norm.device != dev or norm.dtype != torch.float32 or norm.numel() != 1:
-        raise ValueError(f"norm must be one float32 on {dev}")
-    with _On(dev, stream) as s:
-        _check(lib().mcke_sm100_clip_grads(arr, n, max_norm, norm.data_ptr(), s))
+    arr = _grad_list(grads, grads if out is None else out)
+    _one_float(norm, grads[0])
+    if _elsewhere(norm, stream):
+        with _on(norm, stream):
+            return clip_grads(grads, max_norm, norm, out)
+    _check(lib().mcke_sm100_clip_grads(arr, len(grads), max_norm, norm.data_ptr(), _current(norm)))
 
 
 class GemmAttrs(ctypes.Structure):
