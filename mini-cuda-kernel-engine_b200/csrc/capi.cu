@@ -60,6 +60,7 @@ bool pdl_enabled() {
 int read_tc_watchdog(uint32_t* site);
 int launch_watchdog_selftest(cudaStream_t s);
 int read_reduce_watchdog(uint32_t* site);
+int read_layer_norm_watchdog(uint32_t* site);
 
 namespace {
 
@@ -160,7 +161,10 @@ extern "C" int mcke_sm100_check_device_errors(mcke_stream_t stream) {
   if (site != 0)
     return fail(MCKE_INTERNAL,
                 "reduce (one-kernel step): a CTA's partial did not arrive within 1 s; the result is incomplete");
-return MCKE_OK;
+  MCKE_RETURN_IF(read_layer_norm_watchdog(&site));
+  if (site != 0)
+    return fail(MCKE_INTERNAL, "layer norm (backward): a row's sums did not arrive within 2 s; the result is incomplete");
+  return MCKE_OK;
 }
 
 extern "C" int mcke_sm100_watchdog_selftest(mcke_stream_t stream) {

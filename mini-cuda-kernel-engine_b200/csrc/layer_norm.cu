@@ -17,6 +17,10 @@
 namespace mcke_sm100 {
 namespace {
 
+// One persistent block on each SM of a B200, a constant so that results do not
+// depend on the device.
+constexpr int64_t kStreamBlocks = 148;
+
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 
@@ -491,9 +495,144 @@ struct BackwardArgs {
   int rows, cols;
 };
 
+// ---- sums that are posted and collected -----------------------------------------
+//
+// The backward pass splits its sum over a row's warps in two: a warp posts its
+// share and goes on with the row before it while the others' arrive.  Each warp
+// leaves its share in the shared memory of every block of the cluster and arrives on
+// that block's barrier; behind it eight lanes per value add the shares up.
+// Four places take turns.  A warp posts row j + 4 behind its collection of row
+// j + 2, which every warp posted behind its collection of row j: nobody still
+// reads the place of row j.
+constexpr int kPlaces = 4;
+constexpr unsigned long long kWaitNs = 2000000000ull;
+__device__ uint32_t g_layer_norm_watchdog;
+
+template <int kN, int kW, int kCluster>
+struct PostedSums {
+  static_assert(kN == 2 || kN == 4, "values");
+  static constexpr int kEntries = kW * kCluster;  // shares per value
+  static constexpr int kPerLane = (kEntries + 7) / 8;
+  float share[kPlaces][kN][8 * kPerLane];
+  uint64_t arrived[kPlaces];
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t block) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(address), "r"(block));
+  return r;
+}
+
+// By one thread, before any warp of the cluster posts.
+template <int kN, int kW, int kCluster>
+__device__ __forceinline__ void init_sums(PostedSums<kN, kW, kCluster>& p) {
+  for (int k = 0; k < kPlaces; ++k)
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&p.arrived[k])), "r"(kW) : "memory");
+}
+
+// Sums kN values over the warp; value i is left in lanes i * 32 / kN on.
+template <int kN>
+__device__ __forceinline__ float warp_sums(const float (&v)[kN]) {
+  const int lane = threadIdx.x & 31;
+  const bool up = lane & 16;
+  float a;
+  if constexpr (kN == 4) {
+    const bool right = lane & 8;
+    a = (up ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
+    const float b = (up ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+    a = (right ? b : a) + __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
+  } else {
+    a = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
+  }
+#pragma unroll
+  for (int o = 16 / kN; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
+
+// Posts a warp's shares of kN values to place k.
+template <int kN, int kW, int kCluster>
+__device__ __forceinline__ void post_sums(const float (&v)[kN], PostedSums<kN, kW, kCluster>& p, int k) {
+  constexpr int kLanes = 32 / kN;
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % kW;
+  const float a = warp_sums(v);
+  const uint32_t bar = shared_address(&p.arrived[k]);
+  if constexpr (kCluster == 1) {
+    if (lane % kLanes == 0) p.share[k][lane / kLanes][warp] = a;
+    __syncwarp();
+    if (lane == 0) asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  } else {
+    // the first kCluster lanes of each value store it into those blocks; the stores
+    // complete on the barrier there
+    const uint32_t to = lane % kLanes;
+    if (to < kCluster) {
+      const uint32_t at = shared_address(&p.share[k][lane / kLanes][block_in_cluster() * kW + warp]);
+      asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(in_block(at, to)),
+                   "r"(__float_as_uint(a)), "r"(in_block(bar, to))
+                   : "memory");
+    }
+    // this block's warps arrive; the first of them says how many bytes are to come
+    if (lane == 0) {
+      if (warp == 0)
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar),
+                     "n"(kN * 4 * PostedSums<kN, kW, kCluster>::kEntries)
+                     : "memory");
+      else
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+    }
+  }
+}
+
+__device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t phase) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done)
+      : "r"(bar), "r"(phase)
+      : "memory");
+  return done != 0;
+}
+
+// Waits (2 s at most; a wait that runs out is recorded and passed, and the sums are
+// then incomplete) until every share of place k is there, and returns the sums: the
+// same bits in every thread.
+template <int kN, int kW, int kCluster>
+__device__ __forceinline__ void collect_sums(float (&v)[kN], const PostedSums<kN, kW, kCluster>& p, int k,
+                                             uint32_t phase) {
+  const uint32_t bar = shared_address(&p.arrived[k]);
+  if (!try_phase(bar, phase)) {
+    unsigned long long t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    while (!try_phase(bar, phase)) {
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t - t0 > kWaitNs) {
+        atomicCAS(&g_layer_norm_watchdog, 0u, 1u);
+        break;
+      }
+    }
+  }
+  using P = PostedSums<kN, kW, kCluster>;
+  const int lane = threadIdx.x & 31, at = (lane & 7) * P::kPerLane;
+  const float* mine = p.share[k][(lane >> 3) % kN] + at;
+  float a = 0.0f;
+#pragma unroll
+  for (int i = 0; i < P::kPerLane; ++i)
+    if (at + i < P::kEntries) a += mine[i];
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+#pragma unroll
+  for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
+}
+
 // dx, and the column sums of each slab (the rows of one cluster), in one read of dy
 // and x: a thread adds up its 16 columns in registers over all its rows, the
-// block's groups are added in shared memory at the end.  kRows rows at a time.
+// block's groups are added in shared memory at the end.  Each turn of the loop
+// posts the sums of kRows rows and writes dx of the rows of the turn before, whose
+// units are read a second time from the ring.
 template <class T, int kW, int kGroups, int kCluster, int kRows, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kernel(const BackwardArgs a) {
   pdl_entry();
@@ -501,31 +640,42 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
   constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
   using S = Stream<T, kUnits, kW, kGroups, kStages, 2 * kRows>;
   extern __shared__ __align__(16) uint4 ring[];
-  __shared__ GroupSums<2 * kRows, kW, kCluster> red[kGroups];
+  __shared__ PostedSums<2 * kRows, kW, kCluster> posted[kGroups];
   constexpr int kTpr = S::kTpg * kCluster;
   const int group = threadIdx.x / S::kTpg;
   const int t = threadIdx.x % S::kTpg + (kCluster > 1 ? static_cast<int>(block_in_cluster()) * S::kTpg : 0);
   auto live = [&](int i) { return kFull || (i * kTpr + t) * kPer < a.cols; };
-  uint4* const mine = ring + threadIdx.x;
+  // rows kRows p .. of the turn's p = cluster + clusters * (group + kGroups * turn)
   const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
   const int step = kRows * clusters * kGroups;
   int row = kRows * (cluster + clusters * group);
-  if constexpr (kCluster > 1) cluster_barrier();  // every block of it runs before one stores into another
+  if (threadIdx.x % S::kTpg == 0) init_sums(posted[group]);
+  if constexpr (kCluster > 1) {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    cluster_barrier();  // every block of it runs, its barriers in place, before one posts into another
+  } else {
+    __syncthreads();
+  }
   int ahead_row = row;
   const T* dy_ahead = static_cast<const T*>(a.dy) + row * a.dy_stride + t * kPer;
   const T* x_ahead = static_cast<const T*>(a.x) + row * a.x_stride + t * kPer;
-  auto slot = [&](int stage, int k, int operand, int i) {
-    return mine + (((stage * kRows + k) * 2 + operand) * kUnits + i) * S::kThreads;
+  constexpr int kStage = 2 * kRows * kUnits * S::kThreads;  // units of a stage
+  auto slot = [&](uint4* stage, int k, int operand, int i) {
+    return stage + ((k * 2 + operand) * kUnits + i) * S::kThreads;
   };
-  auto fetch = [&](int stage) {
+  uint4* const first_stage = ring + threadIdx.x;
+  uint4* const end_stage = first_stage + kStages * kStage;
+  auto after = [&](uint4* stage) { return stage + kStage == end_stage ? first_stage : stage + kStage; };
+  uint4 *stage = first_stage, *last_stage = first_stage, *ahead_stage = first_stage;
+  auto fetch = [&]() {
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
       if (ahead_row + k < a.rows) {
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
           if (live(i)) {
-            copy_unit_async(slot(stage, k, 0, i), dy_ahead + k * a.dy_stride + i * kTpr * kPer);
-            copy_unit_async(slot(stage, k, 1, i), x_ahead + k * a.x_stride + i * kTpr * kPer);
+            copy_unit_async(slot(ahead_stage, k, 0, i), dy_ahead + k * a.dy_stride + i * kTpr * kPer);
+            copy_unit_async(slot(ahead_stage, k, 1, i), x_ahead + k * a.x_stride + i * kTpr * kPer);
           }
         }
       }
@@ -534,9 +684,10 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
     dy_ahead += step * a.dy_stride;
     x_ahead += step * a.x_stride;
     ahead_row += step;
+    ahead_stage = after(ahead_stage);
   };
 #pragma unroll
-  for (int k = 0; k < kStages - 1; ++k) fetch(k);
+  for (int k = 0; k < kStages - 2; ++k) fetch();
   F2 w[kUnits][kPairs], dw[kUnits][kPairs], db[kUnits][kPairs];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
@@ -545,10 +696,9 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
     for (int j = 0; j < kPairs; ++j) dw[i][j] = db[i][j] = f2(0.0f);
   }
   const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
-  int parity = 0, stage = 0;
   T* dxr = static_cast<T*>(a.dx) + row * a.dx_stride + t * kPer;
-  // the statistics of the rows to come, a step ahead
-  float mu[kRows], r[kRows], next_mu[kRows], next_r[kRows];
+  // the statistics of this turn's rows, of the last turn's and of the next one's
+  float mu[kRows], r[kRows], last_mu[kRows], last_r[kRows], next_mu[kRows], next_r[kRows];
   auto stats = [&](int first, float (&m)[kRows], float (&s)[kRows]) {
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
@@ -557,65 +707,73 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
     }
   };
   stats(row, mu, r);
-  for (; row < a.rows; row += step) {
-    fetch(stage == 0 ? kStages - 1 : stage - 1);
+  // one turn past the last rows: what is posted is collected a turn later
+  for (int turn = 0; row < a.rows + step; ++turn, row += step) {
     stats(row + step, next_mu, next_r);
-    copies_wait<kStages - 1>();
-    uint4 dyq[kRows][kUnits], xq[kRows][kUnits];
-    float sums[2 * kRows];
+    fetch();
+    copies_wait<kStages - 2>();
+    if (row < a.rows) {
+      float sums[2 * kRows];
 #pragma unroll
-    for (int k = 0; k < kRows; ++k) {
-      const F2 minus_mu = f2(-mu[k]), rr = f2(r[k]);
-      F2 s1 = f2(0.0f), s2 = f2(0.0f);
+      for (int k = 0; k < kRows; ++k) {
+        const F2 minus_mu = f2(-mu[k]), rr = f2(r[k]);
+        F2 s1 = f2(0.0f), s2 = f2(0.0f);
 #pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        const bool there = row + k < a.rows && live(i);
-        dyq[k][i] = there ? *slot(stage, k, 0, i) : no_unit();
-        xq[k][i] = there ? *slot(stage, k, 1, i) : no_unit();
-        F2 d[kPairs], v[kPairs];
-        U::pairs(dyq[k][i], d);
-        U::pairs(xq[k][i], v);
+        for (int i = 0; i < kUnits; ++i) {
+          if (!live(i) || (kRows > 1 && row + k >= a.rows)) continue;
+          F2 d[kPairs], v[kPairs];
+          U::pairs(*slot(stage, k, 0, i), d);
+          U::pairs(*slot(stage, k, 1, i), v);
 #pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          const F2 xh = mul2(add2(v[j], minus_mu), rr), g = mul2(d[j], w[i][j]);
-          db[i][j] = add2(db[i][j], d[j]);
-          dw[i][j] = fma2(d[j], xh, dw[i][j]);
-          s1 = add2(s1, g);
-          s2 = fma2(g, xh, s2);
+          for (int j = 0; j < kPairs; ++j) {
+            const F2 dev = add2(v[j], minus_mu), p = mul2(d[j], dev);
+            db[i][j] = add2(db[i][j], d[j]);
+            dw[i][j] = fma2(p, rr, dw[i][j]);
+            s1 = fma2(d[j], w[i][j], s1);
+            s2 = fma2(p, w[i][j], s2);
+          }
+        }
+        sums[2 * k] = sum2(s1);
+        sums[2 * k + 1] = sum2(s2);
+      }
+      post_sums(sums, posted[group], turn % kPlaces);
+    }
+    if (turn > 0) {
+      float c[2 * kRows];
+      collect_sums(c, posted[group], (turn - 1) % kPlaces, static_cast<uint32_t>((turn - 1) / kPlaces) & 1u);
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        if (kRows > 1 && row - step + k >= a.rows) break;
+        // dx = r dy w - r c1 - (x - mu) r^2 c2, the second sum being r short of c2's
+        const F2 minus_mu = f2(-last_mu[k]), rr = f2(last_r[k]);
+        const F2 k1 = f2(-last_r[k] * div_by(c[2 * k], n, inv_n));
+        const F2 k2 = f2(-last_r[k] * last_r[k] * (last_r[k] * div_by(c[2 * k + 1], n, inv_n)));
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          if (!live(i)) continue;
+          F2 d[kPairs], v[kPairs];
+          U::pairs(*slot(last_stage, k, 0, i), d);
+          U::pairs(*slot(last_stage, k, 1, i), v);
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j)
+            v[j] = fma2(add2(v[j], minus_mu), k2, fma2(mul2(d[j], w[i][j]), rr, k1));
+          U::store_pairs(dxr + k * a.dx_stride + i * kTpr * kPer, v);
         }
       }
-      sums[2 * k] = sum2(s1);
-      sums[2 * k + 1] = sum2(s2);
+      dxr += step * a.dx_stride;
     }
-    stage = stage + 1 == kStages ? 0 : stage + 1;
-    group_all_sum(sums, red[group], parity, group);
 #pragma unroll
     for (int k = 0; k < kRows; ++k) {
-      if (row + k >= a.rows) break;
-      const F2 minus_mu = f2(-mu[k]), rr = f2(r[k]);
-      const F2 minus_c1 = f2(-div_by(sums[2 * k], n, inv_n)), minus_c2 = f2(-div_by(sums[2 * k + 1], n, inv_n));
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-        if (!live(i)) continue;
-        F2 d[kPairs], v[kPairs];
-        U::pairs(dyq[k][i], d);
-        U::pairs(xq[k][i], v);
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          const F2 xh = mul2(add2(v[j], minus_mu), rr);
-          v[j] = mul2(fma2(xh, minus_c2, fma2(d[j], w[i][j], minus_c1)), rr);
-        }
-        U::store_pairs(dxr + k * a.dx_stride + i * kTpr * kPer, v);
-      }
-    }
-    dxr += step * a.dx_stride;
-#pragma unroll
-    for (int k = 0; k < kRows; ++k) {
+      last_mu[k] = mu[k];
+      last_r[k] = r[k];
       mu[k] = next_mu[k];
       r[k] = next_r[k];
     }
+    last_stage = stage;
+    stage = after(stage);
   }
   copies_wait<0>();
+  if constexpr (kCluster > 1) cluster_barrier();  // no block leaves while another's post may be on its way to it
   if (!a.part) return;
   // the groups' column sums, added in group order
   if constexpr (kGroups > 1) {
@@ -742,29 +900,32 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // dw and db from the slabs' partial sums [slabs][2 cols]; zeros for no slab.  A block
-// folds 32 columns: warp w adds slabs w, w + kWarps, ... in order, then the warps are
-// added in order.
-__global__ void __launch_bounds__(kThreads)
+// folds 32 columns: warp w adds slabs w, w + 32, ... in order, all of them in flight at
+// once, then the warps are added in order.
+constexpr int kFoldWarps = 32;
+__global__ void __launch_bounds__(32 * kFoldWarps)
     layer_norm_fold_kernel(const float* __restrict__ part, int slabs, float* __restrict__ dweight,
                            float* __restrict__ dbias, int cols) {
   pdl_entry();
-  __shared__ float red[kWarps][32];
+  __shared__ float red[kFoldWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;  // of 2 cols
+  const int64_t width = 2 * static_cast<int64_t>(cols), c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   float s = 0.0f;
-  if (c < 2 * static_cast<int64_t>(cols)) {
-#pragma unroll 4
-    for (int k = warp; k < slabs; k += kWarps) s += part[k * 2 * static_cast<int64_t>(cols) + c];
+  if (c < width) {
+#pragma unroll
+    for (int k = 0; k < (kStreamBlocks + kFoldWarps - 1) / kFoldWarps; ++k)
+      if (warp + k * kFoldWarps < slabs) s += part[(warp + k * kFoldWarps) * width + c];
   }
   red[warp][lane] = s;
   __syncthreads();
-  if (warp > 0 || c >= 2 * static_cast<int64_t>(cols)) return;
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) s += red[w][lane];
-  if (c < cols) {
-    if (dweight) dweight[c] = s;
+  // warp w sums up column w of the 32, a lane per warp's share
+  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + warp;
+  s = warp_all_sum(red[lane][warp]);
+  if (lane > 0 || mine >= width) return;
+  if (mine < cols) {
+    if (dweight) dweight[mine] = s;
   } else if (dbias) {
-    dbias[c - cols] = s;
+    dbias[mine - cols] = s;
   }
 }
 
@@ -783,13 +944,9 @@ bool whole_units(std::initializer_list<const void*> tensors, std::initializer_li
 // row is then spread over as many threads as it has units.
 constexpr int64_t kFewRows = 4 * 148;
 
-// One persistent block on each SM of a B200, a constant so that results do not
-// depend on the device.
-constexpr int64_t kStreamBlocks = 148;
-
 // Slabs of rows whose column sums are kept apart.  From the extents alone, so
 // the order of the sums, and every bit of dw and db, is the same on any GPU.
-int64_t column_slabs(int64_t rows) { return rows < 148 ? rows : 148; }
+int64_t column_slabs(int64_t rows) { return rows < kStreamBlocks ? rows : kStreamBlocks; }
 
 // Calls f with the smallest of the unit counts kUnits, 2 kUnits .. kMax that holds n
 // units over `threads` threads, and with whether they are filled.
@@ -926,7 +1083,8 @@ void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
 // Returns the number of slabs of partial sums that were written.
 template <class T>
 int64_t launch_backward_stream(const BackwardArgs& a, cudaStream_t s) {
-  // f32 rows take twice the ring: one at a time
+  // two bf16 rows a turn halve what a turn costs besides their elements; two f32 rows
+  // would not leave the ring three stages
   constexpr int kRows = sizeof(T) == 2 ? 2 : 1, kStages = 3;
   int64_t slabs = 0;
   with_group(a.cols, [&](auto warps, auto blocks) {
@@ -963,11 +1121,27 @@ void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* d
     }
   }
   if (dweight || dbias)
-    launch_async(layer_norm_fold_kernel, static_cast<unsigned>((2 * static_cast<int64_t>(a.cols) + 31) / 32), kThreads,
-                 0, s, static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
+    launch_async(layer_norm_fold_kernel, static_cast<unsigned>((2 * static_cast<int64_t>(a.cols) + 31) / 32),
+                 32 * kFoldWarps, 0, s, static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
 }
 
 }  // namespace
+}  // namespace mcke_sm100
+
+namespace mcke_sm100 {
+// Reads and clears the word that an expired wait of the backward pass sets.
+int read_layer_norm_watchdog(uint32_t* site) {
+  uint32_t v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_layer_norm_watchdog, sizeof(v));
+  if (e != cudaSuccess) return fail(MCKE_CUDA_ERROR, "watchdog read: %s", cudaGetErrorString(e));
+  if (v != 0) {
+    const uint32_t zero = 0;
+    e = cudaMemcpyToSymbol(g_layer_norm_watchdog, &zero, sizeof(zero));
+    if (e != cudaSuccess) return fail(MCKE_CUDA_ERROR, "watchdog clear: %s", cudaGetErrorString(e));
+  }
+  *site = v;
+  return MCKE_OK;
+}
 }  // namespace mcke_sm100
 
 using namespace mcke_sm100;
