@@ -281,43 +281,13 @@ __device__ __forceinline__ void copies_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
 }
 
-// Sums over a group of kW warps (of each of the kCluster blocks that share a row), of
-// kN = 2 or 4 values at once: the same bits in every thread.  The values part
-// ways on the first exchanges (of four, 16 lanes go on with two each, then 8
-// lanes with one), so four cost six shuffles.  Each warp leaves its sums in the
-// shared memory of every block of the cluster; behind the barrier eight lanes per
-// value add them up.  The two halves of `red` take turns, so a thread that still
-// reads one is never overtaken (the next write to it comes behind the other
-// half's barrier).
-template <int kN, int kW, int kCluster>
-struct GroupSums {
-  static constexpr int kEntries = kW * kCluster;                  // per value
-  static constexpr int kPerLane = (kEntries + 7) / 8;
-  float part[2][kN][8 * kPerLane];
-};
-
-__device__ __forceinline__ void store_in_block(float* p, uint32_t block, float v) {
-  uint32_t at = static_cast<uint32_t>(__cvta_generic_to_shared(p));
-  asm volatile("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(block));
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory");
-}
-__device__ __forceinline__ uint32_t block_in_cluster() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-
-template <int kN, int kW, int kCluster>
-__device__ __forceinline__ void group_all_sum(float (&v)[kN], GroupSums<kN, kW, kCluster>& red, int& parity, int group) {
-  static_assert(kN == 2 || kN == 4, "values");
-  using R = GroupSums<kN, kW, kCluster>;
+// Sums kN values over the warp; value i is left in lanes i * 32 / kN on.  The values
+// part ways on the first exchanges (of four, 16 lanes go on with two each, then 8
+// lanes with one), so four cost six shuffles.
+template <int kN>
+__device__ __forceinline__ float warp_sums(const float (&v)[kN]) {
   const int lane = threadIdx.x & 31;
   const bool up = lane & 16;
-  constexpr int kLanes = 32 / kN;  // that go on with one value
   float a;
   if constexpr (kN == 4) {
     const bool right = lane & 8;
@@ -328,58 +298,60 @@ __device__ __forceinline__ void group_all_sum(float (&v)[kN], GroupSums<kN, kW, 
     a = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
   }
 #pragma unroll
-  for (int o = kLanes / 2; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  if constexpr (kW * kCluster > 1) {
-    float(*r)[8 * R::kPerLane] = red.part[parity];
+  for (int o = 16 / kN; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
+  return a;
+}
+
+// Sums of four values over a group of kW warps at once: the same bits in every
+// thread.  Behind the group's barrier eight lanes per value add the warps' sums
+// up.  The two halves take turns, so a thread that still reads one is never
+// overtaken (the next write to it comes behind the other half's barrier).
+template <int kW>
+struct GroupSums {
+  static constexpr int kPerLane = (kW + 7) / 8;
+  float part[2][4][8 * kPerLane];
+};
+template <int kW>
+__device__ __forceinline__ void group_all_sum(float (&v)[4], GroupSums<kW>& red, int& parity, int group) {
+  const int lane = threadIdx.x & 31;
+  float a = warp_sums(v);
+  if constexpr (kW > 1) {
+    float(*r)[8 * GroupSums<kW>::kPerLane] = red.part[parity];
     parity ^= 1;
-    const int warp = (threadIdx.x >> 5) % kW;
-    if constexpr (kCluster == 1) {
-      if (lane % kLanes == 0) r[lane / kLanes][warp] = a;
-      asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * kW) : "memory");
-    } else {
-      const int entry = block_in_cluster() * kW + warp;
-      if (lane % kLanes < kCluster) store_in_block(&r[lane / kLanes][entry], lane % kLanes, a);
-      cluster_barrier();
-    }
-    const int at = (lane & 7) * R::kPerLane;
-    const float* mine = r[(lane >> 3) % kN] + at;
+    if ((lane & 7) == 0) r[lane >> 3][(threadIdx.x >> 5) % kW] = a;
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(32 * kW) : "memory");
+    const int at = (lane & 7) * GroupSums<kW>::kPerLane;
+    const float* mine = r[lane >> 3] + at;
     a = 0.0f;
 #pragma unroll
-    for (int i = 0; i < R::kPerLane; ++i)
-      if (at + i < R::kEntries) a += mine[i];
+    for (int i = 0; i < GroupSums<kW>::kPerLane; ++i)
+      if (at + i < kW) a += mine[i];
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
-  } else {
-#pragma unroll
-    for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, kLanes * i);
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
 }
 
 // Two rows at a time, 16 elements of each to a thread; the sums of the next two
 // rows and the squared deviations of the current two are reduced together, so
 // two rows cost one barrier and six shuffles although each variance is taken
 // about its row's exact mean.
-template <class T, int kW, int kGroups, int kCluster, int kStages, bool kFull>
+template <class T, int kW, int kGroups, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel(const ForwardArgs a) {
   pdl_entry();
   using U = Unit<T>;
   constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
   using S = Stream<T, kUnits, kW, kGroups, kStages, 2>;
   extern __shared__ __align__(16) uint4 ring[];
-  __shared__ GroupSums<4, kW, kCluster> red[kGroups];
-  // the thread within the row's threads of all blocks; they are kTpr
-  constexpr int kTpr = S::kTpg * kCluster;
-  const int group = threadIdx.x / S::kTpg;
-  const int t = threadIdx.x % S::kTpg + (kCluster > 1 ? static_cast<int>(block_in_cluster()) * S::kTpg : 0);
+  __shared__ GroupSums<kW> red[kGroups];
+  constexpr int kTpr = S::kTpg;
+  const int group = threadIdx.x / S::kTpg, t = threadIdx.x % S::kTpg;
   auto live = [&](int i) { return kFull || (i * kTpr + t) * kPer < a.cols; };
   uint4* const mine = ring + threadIdx.x;
-  // rows 2 p and 2 p + 1 of pair p = cluster + clusters * (group + kGroups * j)
-  const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
-  const int step = 2 * clusters * kGroups;
-  int row = 2 * (cluster + clusters * group);
-  if constexpr (kCluster > 1) cluster_barrier();  // every block of it runs before one stores into another
+  // rows 2 p and 2 p + 1 of pair p = blockIdx.x + gridDim.x * (group + kGroups * j)
+  const int step = 2 * gridDim.x * kGroups;
+  int row = 2 * (blockIdx.x + gridDim.x * group);
   int ahead_row = row;
   const T* ahead = static_cast<const T*>(a.x) + ahead_row * a.x_stride + t * kPer;
   auto fetch = [&](int stage) {
@@ -481,24 +453,20 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel
   copies_wait<0>();
 }
 
-struct BackwardArgs {
-  const void* dy;
-  int64_t dy_stride;
-  const void* x;
-  int64_t x_stride;
-  const float* weight;
-  const float* mean;
-  const float* rstd;
-  void* dx;
-  int64_t dx_stride;
-  float* part;  // [slabs][dw, db][cols], or null: no parameter gradients are wanted
-  int rows, cols;
-};
+__device__ __forceinline__ uint32_t block_in_cluster() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 
 // ---- sums that are posted and collected -----------------------------------------
 //
-// The backward pass splits its sum over a row's warps in two: a warp posts its
-// share and goes on with the row before it while the others' arrive.  Each warp
+// A sum over a row's warps comes in two parts: a warp posts its share and goes on
+// with other rows while the others' arrive, and collects the sum later.  Each warp
 // leaves its share in the shared memory of every block of the cluster and arrives on
 // that block's barrier; behind it eight lanes per value add the shares up.
 // Four places take turns.  A warp posts row j + 4 behind its collection of row
@@ -531,25 +499,6 @@ template <int kN, int kW, int kCluster>
 __device__ __forceinline__ void init_sums(PostedSums<kN, kW, kCluster>& p) {
   for (int k = 0; k < kPlaces; ++k)
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&p.arrived[k])), "r"(kW) : "memory");
-}
-
-// Sums kN values over the warp; value i is left in lanes i * 32 / kN on.
-template <int kN>
-__device__ __forceinline__ float warp_sums(const float (&v)[kN]) {
-  const int lane = threadIdx.x & 31;
-  const bool up = lane & 16;
-  float a;
-  if constexpr (kN == 4) {
-    const bool right = lane & 8;
-    a = (up ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
-    const float b = (up ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
-    a = (right ? b : a) + __shfl_xor_sync(0xffffffffu, right ? a : b, 8);
-  } else {
-    a = (up ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, up ? v[0] : v[1], 16);
-  }
-#pragma unroll
-  for (int o = 16 / kN; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
-  return a;
 }
 
 // Posts a warp's shares of kN values to place k.
@@ -627,6 +576,158 @@ __device__ __forceinline__ void collect_sums(float (&v)[kN], const PostedSums<kN
 #pragma unroll
   for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
 }
+
+// Rows over the blocks of a cluster.  The statistics take two exchanges, the mean's and that of the squared deviations
+// about it, and both ride in one post: turn p collects what turn p - 1 posted (the
+// means of rows p, the variances of rows p - 1), posts the sums of rows p + 1 and
+// the squared deviations of rows p, and writes rows p - 1 while they arrive.  "Rows
+// p" are kRows rows; each is read from the ring in three turns running.
+template <class T, int kW, int kCluster, int kRows, int kStages, bool kFull>
+__global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const ForwardArgs a) {
+  pdl_entry();
+  using U = Unit<T>;
+  constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
+  using S = Stream<T, kUnits, kW, 1, kStages, kRows>;
+  extern __shared__ __align__(16) uint4 ring[];
+  __shared__ PostedSums<2 * kRows, kW, kCluster> posted;
+  constexpr int kTpr = S::kTpg * kCluster;  // the row's threads of all blocks
+  const int t = threadIdx.x + static_cast<int>(block_in_cluster()) * S::kTpg;
+  auto live = [&](int i) { return kFull || (i * kTpr + t) * kPer < a.cols; };
+  const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
+  const int step = kRows * clusters;
+  int row = kRows * cluster;
+  if (threadIdx.x == 0) init_sums(posted);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  cluster_barrier();  // every block of it runs, its barriers in place, before one posts into another
+  int ahead_row = row;
+  const T* ahead = static_cast<const T*>(a.x) + row * a.x_stride + t * kPer;
+  constexpr int kStage = kRows * kUnits * S::kThreads;  // units of a stage
+  auto slot = [&](uint4* stage, int k, int i) { return stage + (k * kUnits + i) * S::kThreads; };
+  uint4* const first_stage = ring + threadIdx.x;
+  uint4* const end_stage = first_stage + kStages * kStage;
+  auto after = [&](uint4* stage) { return stage + kStage == end_stage ? first_stage : stage + kStage; };
+  uint4 *ahead_stage = first_stage, *next_stage = first_stage, *stage = first_stage, *last_stage = first_stage;
+  auto fetch = [&]() {
+#pragma unroll
+    for (int k = 0; k < kRows; ++k) {
+      if (ahead_row + k < a.rows) {
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i)
+          if (live(i)) copy_unit_async(slot(ahead_stage, k, i), ahead + k * a.x_stride + i * kTpr * kPer);
+      }
+    }
+    copies_commit();
+    ahead += step * a.x_stride;
+    ahead_row += step;
+    ahead_stage = after(ahead_stage);
+  };
+#pragma unroll
+  for (int k = 0; k < kStages - 2; ++k) fetch();
+  F2 w[kUnits][kPairs], b[kUnits][kPairs];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    load_param_pairs<kPer>(live(i) ? a.weight : nullptr, (i * kTpr + t) * kPer, 1.0f, w[i]);
+    load_param_pairs<kPer>(live(i) ? a.bias : nullptr, (i * kTpr + t) * kPer, 0.0f, b[i]);
+  }
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  T* yr = static_cast<T*>(a.y) + row * a.y_stride + t * kPer;
+  float mu[kRows], last_mu[kRows];
+#pragma unroll
+  for (int k = 0; k < kRows; ++k) mu[k] = 0.0f;
+  row -= step;
+  // turns p = -1 (it posts the first sums) to one past the last rows
+  for (int turn = 0; row < a.rows + step; ++turn, row += step) {
+    float c[2 * kRows];
+#pragma unroll
+    for (int i = 0; i < 2 * kRows; ++i) c[i] = 0.0f;
+    if (turn > 0) {
+      collect_sums(c, posted, (turn - 1) % kPlaces, static_cast<uint32_t>((turn - 1) / kPlaces) & 1u);
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        last_mu[k] = mu[k];
+        mu[k] = div_by(c[k], n, inv_n);
+      }
+    }
+    if (turn > 0) fetch();
+    copies_wait<kStages - 3>();
+    if (row < a.rows) {
+      float sums[2 * kRows];
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        F2 s = f2(0.0f), d2 = f2(0.0f);
+        if (row + step + k < a.rows) {
+#pragma unroll
+          for (int i = 0; i < kUnits; ++i) {
+            if (!live(i)) continue;
+            F2 v[kPairs];
+            U::pairs(*slot(next_stage, k, i), v);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) s = add2(s, v[j]);
+          }
+        }
+        if (turn > 0 && row + k < a.rows) {
+          const F2 minus_mu = f2(-mu[k]);
+#pragma unroll
+          for (int i = 0; i < kUnits; ++i) {
+            if (!live(i)) continue;
+            F2 v[kPairs];
+            U::pairs(*slot(stage, k, i), v);
+#pragma unroll
+            for (int j = 0; j < kPairs; ++j) {
+              const F2 d = add2(v[j], minus_mu);
+              d2 = fma2(d, d, d2);
+            }
+          }
+        }
+        sums[k] = sum2(s);
+        sums[kRows + k] = sum2(d2);
+      }
+      post_sums(sums, posted, turn % kPlaces);
+    }
+    if (turn > 1) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int done = row - step + k;
+        if (kRows > 1 && done >= a.rows) break;
+        const float r = rsqrtf(div_by(c[kRows + k], n, inv_n) + a.eps);
+        if (t == 0) {
+          if (a.mean) a.mean[done] = last_mu[k];
+          if (a.rstd) a.rstd[done] = r;
+        }
+        const F2 rr = f2(r), minus_mu = f2(-last_mu[k]);
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          if (!live(i)) continue;
+          F2 v[kPairs];
+          U::pairs(*slot(last_stage, k, i), v);
+#pragma unroll
+          for (int j = 0; j < kPairs; ++j) v[j] = fma2(mul2(add2(v[j], minus_mu), rr), w[i][j], b[i][j]);
+          U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
+        }
+      }
+      yr += step * a.y_stride;
+    }
+    last_stage = stage;
+    stage = next_stage;
+    next_stage = after(next_stage);
+  }
+  copies_wait<0>();
+  cluster_barrier();  // no block leaves while another's post may be on its way to it
+}
+
+struct BackwardArgs {
+  const void* dy;
+  int64_t dy_stride;
+  const void* x;
+  int64_t x_stride;
+  const float* weight;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  int64_t dx_stride;
+  float* part;  // [slabs][dw, db][cols], or null: no parameter gradients are wanted
+  int rows, cols;
+};
 
 // dx, and the column sums of each slab (the rows of one cluster), in one read of dy
 // and x: a thread adds up its 16 columns in registers over all its rows, the
@@ -974,7 +1075,10 @@ int64_t launch_stream(void (*kernel)(const A), const A& a, int64_t items, int th
   // the attribute is a property of the kernel on the current device: set it every time
   cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                        static_cast<int>(smem));
-  const int64_t clusters = items < kStreamBlocks / kCluster ? items : kStreamBlocks / kCluster;
+  // 33 clusters of four fit a B200 (its 148 SMs come in groups that four does not
+  // divide), 74 of two
+  constexpr int64_t kMost = kCluster == 4 ? 32 : kStreamBlocks / kCluster;
+  const int64_t clusters = items < kMost ? items : kMost;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>(clusters * kCluster));
@@ -1022,16 +1126,24 @@ void with_group(int64_t cols, F&& f) {
 
 template <class T>
 void launch_forward_stream(const ForwardArgs& a, cudaStream_t s) {
-  constexpr int kStages = 3;
+  constexpr int kUnits = 16 / Unit<T>::kPer;
   with_group(a.cols, [&](auto warps, auto blocks) {
     constexpr int kW = decltype(warps)::value, kC = decltype(blocks)::value;
-    constexpr int kGroups = kW == 1 ? 15 : 16 / kW;
-    using S = Stream<T, 16 / Unit<T>::kPer, kW, kGroups, kStages, 2>;
+    const bool full = a.cols == 512 * kW * kC;
     const int64_t pairs = (a.rows + 1) / 2;
-    if (a.cols == 512 * kW * kC)
-      launch_stream<kC>(layer_norm_stream_kernel<T, kW, kGroups, kC, kStages, true>, a, pairs, S::kThreads, S::kSmem, s);
-    else
-      launch_stream<kC>(layer_norm_stream_kernel<T, kW, kGroups, kC, kStages, false>, a, pairs, S::kThreads, S::kSmem, s);
+    if constexpr (kC > 1) {
+      constexpr int kRows = sizeof(T) == 2 ? 2 : 1, kStages = 5;
+      using S = Stream<T, kUnits, kW, 1, kStages, kRows>;
+      launch_stream<kC>(full ? layer_norm_cluster_kernel<T, kW, kC, kRows, kStages, true>
+                             : layer_norm_cluster_kernel<T, kW, kC, kRows, kStages, false>,
+                        a, kRows == 2 ? pairs : a.rows, S::kThreads, S::kSmem, s);
+    } else if constexpr (sizeof(T) == 2) {
+      constexpr int kGroups = kW == 1 ? 15 : 16 / kW, kStages = 3;
+      using S = Stream<T, kUnits, kW, kGroups, kStages, 2>;
+      launch_stream<1>(full ? layer_norm_stream_kernel<T, kW, kGroups, kStages, true>
+                            : layer_norm_stream_kernel<T, kW, kGroups, kStages, false>,
+                       a, pairs, S::kThreads, S::kSmem, s);
+    }
   });
 }
 
