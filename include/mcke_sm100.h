@@ -390,13 +390,15 @@ int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride, const void
 /* Of each row of logits: logprobs = the log probability of its target,
  * lse = log(sum(exp)), entropy = -sum(p log p) (natural logarithms), and the
  * top_k likeliest tokens (top_logprobs, top_ids: [rows, top_k], 0 .. MCKE_TOP_MAX
- * of them, by value and among equals by index; NaN above all).  Any of the
+ * of them, by value and among equals by index; NaN above all; of at most
+ * MCKE_TOP_COLS_MAX columns).  Any of the
  * outputs may be NULL (top_k 0).
  * A logit of -inf is a token that cannot come.  A row with nothing else has
  * lse, logprobs and top_logprobs -inf and entropy 0.  A NaN or a +inf makes the
  * row's results NaN.  A negative target is padding: log probability 0.  A target
  * >= cols gives NaN. */
 #define MCKE_TOP_MAX 32
+#define MCKE_TOP_COLS_MAX 4194304
 int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int64_t rows, int64_t cols, int dtype,
                               const int64_t* targets, float* logprobs, float* lse, float* entropy, int top_k,
                               float* top_logprobs, int64_t* top_ids, mcke_stream_t stream);

@@ -21,41 +21,127 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr float kLog2E = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// 16 bytes of a row: kPer elements.  A row is taken in vectors counted from the
+// 16-byte boundary at or below its first element, so rows of any length and start
+// are read in whole aligned vectors; only the first and the last of a row can be
+// partial, and those are read element by element.
+template <class T>
+struct Vec {
+  static constexpr int kPer = 16 / sizeof(T);
+};
+template <class T>
+__device__ __forceinline__ int vec_shift(const T* row) {
+  return static_cast<int>((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+}
+// Plain loads: the backward pass may overwrite the row in place.
+__device__ __forceinline__ uint4 ld_vec(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void unpack(const uint4& q, F2 (&v)[2], const float*) {
+  v[0] = f2(__uint_as_float(q.x), __uint_as_float(q.y));
+  v[1] = f2(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+__device__ __forceinline__ void unpack(const uint4& q, F2 (&v)[4], const uint16_t*) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = f2(bf16_lo(w[j]), bf16_hi(w[j]));
+}
+// Vector of a row that starts at element `first`; -inf where the row has no element.
+template <class T>
+__device__ __forceinline__ uint4 ld_row(const T* row, int64_t first, int64_t cols) {
+  constexpr int kPer = Vec<T>::kPer;
+  if (first >= 0 && first + kPer <= cols) return ld_vec(row + first);
+  uint32_t w[4];
+  constexpr int kPerWord = kPer / 4;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    w[j] = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+#pragma unroll
+    for (int h = 0; h < kPerWord; ++h) {
+      const int64_t c = first + j * kPerWord + h;
+      if (c < 0 || c >= cols) continue;
+      if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(row[c]);
+      else w[j] = (w[j] & (h ? 0x0000ffffu : 0xffff0000u)) | (static_cast<uint32_t>(row[c]) << (16 * h));
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Maxima that keep a NaN, as the sums they belong to do.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t max_nan_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ float vec_max(const uint4& q, const float*) {
+  return max_nan(max_nan(__uint_as_float(q.x), __uint_as_float(q.y)), max_nan(__uint_as_float(q.z), __uint_as_float(q.w)));
+}
+__device__ __forceinline__ float vec_max(const uint4& q, const uint16_t*) {
+  const uint32_t m = max_nan_bf16x2(max_nan_bf16x2(q.x, q.y), max_nan_bf16x2(q.z, q.w));
+  return max_nan(bf16_lo(m), bf16_hi(m));
+}
+__device__ __forceinline__ float exp2_fast(float t) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(t));
+  return r;
+}
+
+// Running statistics of a part of a row: its maximum m, s = sum 2^t and
+// w = sum 2^t t with t = (x - m) log2 e.  Where there is nothing but -inf,
+// m = -inf and s = w = 0.
+struct Stats {
+  float m, s, w;
+};
+// What a maximum of -inf is replaced by, so that x - m is -inf and not NaN.
+__device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
+// The sums of `a` on the scale of a maximum m (>= a.m, finite_max applied).
+__device__ __forceinline__ Stats rescale(const Stats& a, float m) {
+  const float t = a.m == -INFINITY ? 0.0f : (a.m - m) * kLog2E;
+  const float f = exp2_fast(t);
+  // a maximum so far above that nothing is left: f = 0, and t may be -inf
+  return Stats{m, a.s * f, f == 0.0f ? 0.0f : f * fmaf(a.s, t, a.w)};
+}
+__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
+  const float m = max_nan(a.m, b.m);
+  const Stats p = rescale(a, finite_max(m)), q = rescale(b, finite_max(m));
+  return Stats{m, p.s + q.s, p.w + q.w};
+}
 
 // Order of the alternatives: larger value first (NaN above all, -0 equal to
 // +0), then lower index.  Never 0, so 0 stands for "none".
-__device__ __forceinline__ uint64_t order_key(float v, int64_t index) {
-  uint32_t u = __float_as_uint(v + 0.0f);
-  u = (v != v) ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return (static_cast<uint64_t>(u) << 32) | static_cast<uint32_t>(~static_cast<uint32_t>(index));
+__device__ __forceinline__ uint32_t order_key(float v) {
+  const uint32_t u = __float_as_uint(v + 0.0f);
+  return (v != v) ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t key) {
+  return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+__device__ __forceinline__ int64_t key_index(uint64_t key) {
+  return static_cast<uint32_t>(~static_cast<uint32_t>(key));
+}
+// The largest of the warp's 64-bit keys.
+__device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
+  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
+  const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
+  return (static_cast<uint64_t>(hi) << 32) | lo;
 }
 
-__device__ __forceinline__ uint64_t warp_all_max(uint64_t v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const uint64_t w = __shfl_xor_sync(0xffffffffu, v, o);
-    v = w > v ? w : v;
-  }
-  return v;
-}
-__device__ __forceinline__ float warp_all_max(float v) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-// `red` as for block_all_sum.
-template <class V>
-__device__ __forceinline__ V block_all_max(V v, V* red) {
-  v = warp_all_max(v);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  V t = red[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) t = red[w] > t ? red[w] : t;
-  return t;
-}
-
-struct ForwardOut {
+struct ForwardArgs {
+  int64_t stride, cols;
+  const int64_t* targets;
   float* logprobs;
   float* lse;
   float* entropy;
@@ -64,54 +150,233 @@ struct ForwardOut {
   int top_k;
 };
 
-// One block per row: the maximum, the sums, then one pass per alternative.
+__device__ __forceinline__ uint32_t cluster_block() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t cluster_blocks() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t address_in_block(const void* p, uint32_t block) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;"
+               : "=r"(r)
+               : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(block));
+  return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+constexpr int kMaxCluster = 8;
+constexpr int kLoads = 4;  // vectors of a thread in flight
+
+// The k likeliest of a block's part of the row, into best[0 .. k) in order.
+//
+// Every warp load is a chunk of 32 vectors whose maximum the first pass left in
+// chunk_max (a 32-bit order key; chunk c of the part is entry c).  Ordered by
+// maximum and, among equals, by position, the k best chunks hold the k best
+// elements: an element of any other chunk has the k chunks' maxima before it.
+// So one warp picks those chunks, and only they are read again; elements below
+// the k-th chunk's maximum are passed over, and each warp keeps its k best in its
+// lanes, in order.
 template <class T>
-__global__ void __launch_bounds__(kThreads)
-    token_logprobs_row_kernel(const T* __restrict__ x, int64_t stride, int64_t cols,
-                              const int64_t* __restrict__ targets, ForwardOut out) {
+__device__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift, uint32_t* chunk_max, int chunks,
+                            int k, uint64_t (*lists)[MCKE_TOP_MAX], int* picked, uint64_t* best) {
+  constexpr int kPer = Vec<T>::kPer;
+  __shared__ uint32_t threshold;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int n = k < chunks ? k : chunks;
+  if (warp == 0) {
+    uint32_t last = 0;
+    for (int i = 0; i < n; ++i) {
+      uint64_t key = 0;
+      for (int c = lane; c < chunks; c += 32) {
+        const uint64_t e = (static_cast<uint64_t>(chunk_max[c]) << 32) | static_cast<uint32_t>(~c);
+        if (chunk_max[c] != 0u && e > key) key = e;
+      }
+      key = warp_max_key(key);
+      last = static_cast<uint32_t>(key >> 32);
+      const int c = static_cast<int>(~static_cast<uint32_t>(key));
+      if (lane == 0) {
+        picked[i] = c;
+        chunk_max[c] = 0u;
+      }
+      __syncwarp();
+    }
+    if (lane == 0) threshold = n < k ? 1u : last;  // fewer chunks than k: all of their elements count
+  }
+  __syncthreads();
+  uint64_t mine = 0;  // lane l: this warp's l-th best
+  for (int i = warp; i < n; i += kWarps) {
+    const int64_t first = (first_vec + static_cast<int64_t>(picked[i]) * 32 + lane) * kPer - shift;
+    const uint4 q = ld_row(row, first, cols);
+    F2 v[kPer / 2];
+    unpack(q, v, row);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const float x = j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x;
+      const uint32_t value = order_key(x);
+      const bool in_row = first + j >= 0 && first + j < cols;
+      unsigned todo = __ballot_sync(0xffffffffu, in_row && value >= threshold);
+      while (todo) {
+        const int from = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const uint64_t key = (static_cast<uint64_t>(__shfl_sync(0xffffffffu, value, from)) << 32) |
+                             static_cast<uint32_t>(~static_cast<uint32_t>(first + j + (from - lane) * kPer));
+        const int at = __popc(__ballot_sync(0xffffffffu, mine > key));
+        const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
+        if (lane == at) mine = key;
+        else if (lane > at) mine = up;
+      }
+    }
+  }
+  if (lane < k) lists[warp][lane] = mine;
+  __syncthreads();
+  if (warp == 0) {  // lane w walks warp w's list
+    int at = 0;
+    for (int i = 0; i < k; ++i) {
+      const uint64_t head = lane < kWarps && at < k ? lists[lane][at] : 0;
+      const uint64_t key = warp_max_key(head);
+      if (head == key && key != 0) ++at;
+      if (lane == 0) best[i] = key;
+    }
+  }
+}
+
+// A row to each cluster of 1, 2, 4 or 8 blocks, each with a run of the row's chunks:
+// one read of the row with a running maximum and the two sums on its scale; the
+// blocks' results are joined in the first block's shared memory, in order.
+template <class T, bool kEntropy, bool kTop>
+__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ x, const ForwardArgs a) {
   pdl_entry();
-  __shared__ float red[3][kWarps];
-  __shared__ uint64_t red_key[2][kWarps];
-  const int64_t row = blockIdx.x;
-  const T* xr = x + row * stride;
-  float m = -INFINITY;
-  for (int64_t c = threadIdx.x; c < cols; c += kThreads) m = fmaxf(m, ld_val(xr + c));
-  m = block_all_max(m, red[0]);
-  const bool none = m == -INFINITY;
-  float s = 0.0f, w = 0.0f;
-  for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-    const float v = ld_val(xr + c);
-    if (v == -INFINITY) continue;
-    const float d = v - m, e = expf(d);
-    s += e;
-    w += e > 0.0f ? e * d : 0.0f;  // e^d d -> 0
+  constexpr int kPer = Vec<T>::kPer, kPairs = kPer / 2;
+  extern __shared__ uint32_t chunk_max[];
+  __shared__ Stats warp_stats[kWarps];
+  __shared__ Stats part_stats[kMaxCluster];
+  __shared__ uint64_t part_best[kTop ? kMaxCluster : 1][MCKE_TOP_MAX];
+  __shared__ uint64_t lists[kTop ? kWarps : 1][MCKE_TOP_MAX];
+  __shared__ int picked[MCKE_TOP_MAX];
+  const uint32_t blocks = cluster_blocks(), block = cluster_block();
+  const int64_t row = blockIdx.x / blocks;
+  const T* xr = x + row * a.stride;
+  const int shift = vec_shift(xr);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t vecs = (a.cols + shift + kPer - 1) / kPer;
+  const int64_t all_chunks = (vecs + 31) / 32;
+  const int64_t chunk0 = all_chunks * block / blocks, chunk1 = all_chunks * (block + 1) / blocks;
+  const int chunks = static_cast<int>(chunk1 - chunk0);
+
+  Stats st{-INFINITY, 0.0f, 0.0f};
+  for (int c = warp; c < chunks; c += kWarps * kLoads) {
+    uint4 q[kLoads];
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const int64_t v = (chunk0 + c + u * kWarps) * 32 + lane;
+      q[u] = c + u * kWarps < chunks ? ld_row(xr, v * kPer - shift, a.cols)
+                                     : ld_row(xr, a.cols, a.cols);  // past the row: -inf
+    }
+    float m = st.m;
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      const float mu = vec_max(q[u], xr);
+      if constexpr (kTop) {
+        const uint32_t key = __reduce_max_sync(0xffffffffu, order_key(mu));
+        if (lane == 0 && c + u * kWarps < chunks) chunk_max[c + u * kWarps] = key;
+      }
+      m = max_nan(m, mu);
+    }
+    const float mf = finite_max(m);
+    st = rescale(st, mf);
+    st.m = m;
+    const F2 minus_m = f2(-mf), scale = f2(kLog2E);
+    F2 s2 = f2(0.0f), w2 = f2(0.0f);
+#pragma unroll
+    for (int u = 0; u < kLoads; ++u) {
+      F2 v[kPairs];
+      unpack(q[u], v, xr);
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) {
+        float2 t = split(mul2(add2(v[j], minus_m), scale));
+        if constexpr (kEntropy) {
+          // 2^t is 0 long before -200; t itself has to stay finite for 2^t t
+          t.x = max_nan(t.x, -200.0f);
+          t.y = max_nan(t.y, -200.0f);
+        }
+        const F2 e = f2(exp2_fast(t.x), exp2_fast(t.y));
+        s2 = add2(s2, e);
+        if constexpr (kEntropy) w2 = fma2(e, f2(t.x, t.y), w2);
+      }
+    }
+    st.s += sum2(s2);
+    if constexpr (kEntropy) st.w += sum2(w2);
   }
-  s = block_all_sum<kWarps>(s, red[1]);
-  w = block_all_sum<kWarps>(w, red[2]);
-  const float ln_s = logf(s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats other;
+    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    other.w = kEntropy ? __shfl_xor_sync(0xffffffffu, st.w, o) : 0.0f;
+    st = join(st, other);
+  }
+  if (lane == 0) warp_stats[warp] = st;
+  __syncthreads();
+  if constexpr (kTop)
+    top_of_part(xr, a.cols, chunk0 * 32, shift, chunk_max, chunks, a.top_k, lists, picked, part_best[block]);
   if (threadIdx.x == 0) {
-    if (out.lse) out.lse[row] = none ? (s != s ? s : m) : m + ln_s;
-    if (out.entropy) out.entropy[row] = none ? (s != s ? s : 0.0f) : ln_s - w / s;
-    if (out.logprobs) {
-      const int64_t t = targets[row];
-      float lp = 0.0f;
-      if (t >= cols) lp = NAN;
-      else if (t >= 0) lp = none ? (s != s ? s : m) : (ld_val(xr + t) - m) - ln_s;
-      out.logprobs[row] = lp;
+    st = warp_stats[0];
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
+    part_stats[block] = st;
+  }
+  if (blocks > 1) {
+    __syncthreads();
+    cluster_barrier();  // every block of the cluster runs: its shared memory may be written
+    if (block > 0) {
+      const uint32_t to = address_in_block(&part_stats[block], 0);
+      const uint32_t words[3] = {__float_as_uint(part_stats[block].m), __float_as_uint(part_stats[block].s),
+                                 __float_as_uint(part_stats[block].w)};
+      if (threadIdx.x < 3)
+        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * threadIdx.x), "r"(words[threadIdx.x]) : "memory");
+      if (kTop && threadIdx.x < a.top_k)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(address_in_block(&part_best[block][threadIdx.x], 0)),
+                     "l"(part_best[block][threadIdx.x])
+                     : "memory");
+    }
+    cluster_barrier();
+    if (block > 0) return;
+  }
+  if (warp > 0) return;
+  __syncwarp();
+  st = part_stats[0];
+  for (uint32_t b = 1; b < blocks; ++b) st = join(st, part_stats[b]);
+  // a row of which nothing is left (a NaN or +inf makes s NaN: it has no such row)
+  const bool none = st.m == -INFINITY;
+  const float ln_s = logf(st.s);
+  auto logprob = [&](float v) { return none ? -INFINITY : (v - st.m) - ln_s; };
+  if (lane == 0) {
+    if (a.lse) a.lse[row] = none ? -INFINITY : st.m + ln_s;
+    if (kEntropy && a.entropy) a.entropy[row] = none ? 0.0f : ln_s - kLn2 * (st.w / st.s);
+    if (a.logprobs) {
+      const int64_t t = a.targets[row];
+      a.logprobs[row] = t < 0 ? 0.0f : t >= a.cols ? NAN : logprob(ld_val(xr + t));
     }
   }
-  uint64_t last = ~uint64_t{0};
-  for (int k = 0; k < out.top_k; ++k) {
-    uint64_t best = 0;
-    for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-      const uint64_t key = order_key(ld_val(xr + c), c);
-      if (key < last && key > best) best = key;
-    }
-    last = block_all_max(best, red_key[k & 1]);
-    if (threadIdx.x == 0) {
-      const int64_t id = static_cast<uint32_t>(~static_cast<uint32_t>(last));
-      out.top_ids[row * out.top_k + k] = id;
-      out.top_logprobs[row * out.top_k + k] = none ? (s != s ? s : m) : (ld_val(xr + id) - m) - ln_s;
+  if constexpr (kTop) {
+    // lane b walks block b's list
+    int at = 0;
+    for (int i = 0; i < a.top_k; ++i) {
+      const uint64_t head = lane < static_cast<int>(blocks) && at < a.top_k ? part_best[lane][at] : 0;
+      const uint64_t key = warp_max_key(head);
+      if (head == key && key != 0) ++at;
+      if (lane == 0) {
+        a.top_ids[row * a.top_k + i] = key_index(key);
+        a.top_logprobs[row * a.top_k + i] = logprob(key_value(static_cast<uint32_t>(key >> 32)));
+      }
     }
   }
 }
@@ -125,30 +390,146 @@ struct Grads {
   const float* grad_lse;
 };
 
-// dx may be x itself: an element is read before it is written, by the same thread.
-template <class T>
+// dx may be x itself: a vector is read before it is written, by the same thread.
+// A block takes kVecs vectors of a row to a thread; kSame: dx has the row's offset from
+// a 16-byte boundary, so whole vectors are stored.
+constexpr int kVecs = 4;
+template <class T, bool kEntropy, bool kSame>
 __global__ void __launch_bounds__(kThreads)
-    token_logprobs_backward_kernel(const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t cols, Grads g) {
+    token_logprobs_backward_kernel(const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t cols, int parts,
+                                   Grads g) {
   pdl_entry();
-  const int64_t row = blockIdx.x;
+  constexpr int kPer = Vec<T>::kPer, kPairs = kPer / 2;
+  const int64_t row = blockIdx.x / parts;
+  const int64_t part = blockIdx.x - row * parts;
   const T* xr = x + row * stride;
   T* dxr = dx + row * dx_stride;
+  const int shift = vec_shift(xr);
+  int64_t first[kVecs];
+  uint4 q[kVecs];
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    first[u] = ((part * kVecs + u) * kThreads + threadIdx.x) * kPer - shift;
+    q[u] = ld_row(xr, first[u] < cols ? first[u] : cols, cols);
+  }
   const float lse = g.lse[row];
   const int64_t t = g.logprobs ? g.targets[row] : -1;
   const float g_lp = t < 0 ? 0.0f : t >= cols ? NAN : g.logprobs[row];
-  const float g_h = g.grad_entropy ? g.grad_entropy[row] : 0.0f;
-  const float h = g.grad_entropy ? g.entropy[row] : 0.0f;
-  const float a = (g.grad_lse ? g.grad_lse[row] : 0.0f) - g_lp;
-  for (int64_t c = threadIdx.x; c < cols; c += kThreads) {
-    float d = 0.0f;
-    if (lse != -INFINITY) {
-      const float q = ld_val(xr + c) - lse;
-      const float p = expf(q);
-      d = (c == t ? g_lp : 0.0f) + (p == 0.0f ? 0.0f : p * (a - g_h * (q + h)));
-      if (p == 0.0f && a != a) d = a;  // a bad target's NaN reaches every element
+  const float a0 = (g.grad_lse ? g.grad_lse[row] : 0.0f) - g_lp;
+  const float g_h = kEntropy ? g.grad_entropy[row] : 0.0f;
+  // dx = p (a - g_h (q + H)) = p (b - g_h q) besides the target's own term
+  const F2 b = f2(kEntropy ? a0 - g_h * g.entropy[row] : a0), minus_gh = f2(-g_h);
+  const bool none = lse == -INFINITY;
+  const F2 minus_lse = f2(none ? 0.0f : -lse), scale = f2(kLog2E);
+#pragma unroll
+  for (int u = 0; u < kVecs; ++u) {
+    if (first[u] >= cols) continue;
+    F2 v[kPairs];
+    unpack(q[u], v, xr);
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+      float2 d = split(add2(v[j], minus_lse));
+      if constexpr (kEntropy) {
+        // p is 0 long before -150; q itself has to stay finite for p q
+        d.x = max_nan(d.x, -150.0f);
+        d.y = max_nan(d.y, -150.0f);
+      }
+      const F2 dd = f2(d.x, d.y);
+      const float2 e = split(mul2(dd, scale));
+      const F2 p = f2(exp2_fast(e.x), exp2_fast(e.y));
+      v[j] = mul2(p, kEntropy ? fma2(dd, minus_gh, b) : b);
     }
-    st_val(dxr + c, d);
+    const int64_t hit = t - first[u];
+    if (hit >= 0 && hit < kPer && !none) {
+#pragma unroll
+      for (int j = 0; j < kPairs; ++j) v[j] = add2(v[j], f2(hit == 2 * j ? g_lp : 0.0f, hit == 2 * j + 1 ? g_lp : 0.0f));
+    }
+    const bool whole = kSame && first[u] >= 0 && first[u] + kPer <= cols;
+    if constexpr (sizeof(T) == 4) {
+      const float2 lo = split(v[0]), hi = split(v[1]);
+      if (whole) {
+        st_stream_f4(dxr + first[u], make_float4(lo.x, lo.y, hi.x, hi.y));
+        continue;
+      }
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 f = split(v[j]);
+        w[j] = pack_bf16x2(f.x, f.y);
+      }
+      if (whole) {
+        st_stream_u4(dxr + first[u], make_uint4(w[0], w[1], w[2], w[3]));
+        continue;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) {
+      const int64_t c = first[u] + j;
+      if (c >= 0 && c < cols) st_val(dxr + c, j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x);
+    }
   }
+}
+
+// Blocks that share a row.  With few rows a row's time is that of one block's
+// share of it, so the row is spread until the blocks fill the device about once; a
+// block keeps at least a full round of loads.
+template <class T>
+int row_blocks(int64_t rows, int64_t cols) {
+  const int64_t rounds = (cols + kThreads * kLoads * Vec<T>::kPer - 1) / (kThreads * kLoads * Vec<T>::kPer);
+  int n = 1;
+  while (n < kMaxCluster && 2 * n * rows <= 2 * 148 && n < rounds) n *= 2;
+  return n;
+}
+
+template <class T>
+void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
+  const int blocks = row_blocks<T>(rows, a.cols);
+  const bool top = a.top_k > 0;
+  // the largest part's chunk maxima
+  const int64_t chunks = ((a.cols + Vec<T>::kPer - 1) / Vec<T>::kPer + 1 + 31) / 32;
+  const std::size_t smem = top ? static_cast<std::size_t>((chunks + blocks - 1) / blocks + 1) * 4 : 0;
+  auto kernel = a.entropy ? (top ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, true, false>)
+                          : (top ? token_logprobs_kernel<T, false, true> : token_logprobs_kernel<T, false, false>);
+  if (smem > 32 * 1024)
+    cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                         static_cast<int>(smem));
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  cfg.gridDim = dim3(static_cast<unsigned>(rows * blocks));
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(blocks);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.numAttrs = 1;
+  if (pdl_enabled()) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
+  cudaLaunchKernelEx(&cfg, kernel, x, a);  // errors are left for check_launch()
+}
+
+template <class T>
+int launch_backward(const char* who, const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t rows, int64_t cols,
+                    const Grads& g, cudaStream_t s) {
+  constexpr int kPer = Vec<T>::kPer;
+  const int64_t per_block = static_cast<int64_t>(kThreads) * kVecs * kPer;
+  const int64_t parts = (cols + kPer - 1 + per_block - 1) / per_block;  // whatever the row's shift
+  if (rows * parts > 2147483647LL) return fail(MCKE_INVALID_ARGUMENT, "%s: too many elements for one launch", who);
+  const bool same = (reinterpret_cast<std::uintptr_t>(x) - reinterpret_cast<std::uintptr_t>(dx)) % 16 == 0 &&
+                    (rows == 1 || (stride - dx_stride) % kPer == 0);
+  auto kernel = g.grad_entropy ? (same ? token_logprobs_backward_kernel<T, true, true>
+                                       : token_logprobs_backward_kernel<T, true, false>)
+                               : (same ? token_logprobs_backward_kernel<T, false, true>
+                                       : token_logprobs_backward_kernel<T, false, false>);
+  launch_async(kernel, static_cast<unsigned>(rows * parts), kThreads, 0, s, x, stride, dx, dx_stride, cols,
+               static_cast<int>(parts), g);
+  return MCKE_OK;
 }
 
 }  // namespace
@@ -170,6 +551,8 @@ extern "C" int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int
   if (rows > 2147483647LL || cols > 2147483647LL)
     return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX", who);
   if (top_k > cols) return fail(MCKE_INVALID_ARGUMENT, "%s: top_k %d of %lld columns", who, top_k, static_cast<long long>(cols));
+  if (top_k > 0 && cols > MCKE_TOP_COLS_MAX)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: top_k of more than %d columns", who, MCKE_TOP_COLS_MAX);
   if (!logits || (logprobs && !targets) || (top_k > 0 && (!top_logprobs || !top_ids)))
     return fail(MCKE_INVALID_ARGUMENT, "%s: null pointer", who);
   if (!logprobs && !lse && !entropy && top_k == 0) return MCKE_OK;
@@ -183,13 +566,9 @@ extern "C" int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int
   const RowSpan ins[] = {span_of("logits", logits, rows, cols, stride, e), span_of("targets", targets, rows * 8)};
   MCKE_RETURN_IF(check_overlaps(who, outs, ins));
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const ForwardOut out = {logprobs, lse, entropy, top_logprobs, top_ids, top_k};
-  if (dtype == MCKE_DTYPE_BF16)
-    launch_async(token_logprobs_row_kernel<uint16_t>, static_cast<unsigned>(rows), kThreads, 0, s,
-                 static_cast<const uint16_t*>(logits), stride, cols, targets, out);
-  else
-    launch_async(token_logprobs_row_kernel<float>, static_cast<unsigned>(rows), kThreads, 0, s,
-                 static_cast<const float*>(logits), stride, cols, targets, out);
+  const ForwardArgs a = {stride, cols, targets, logprobs, lse, entropy, top_logprobs, top_ids, top_k};
+  if (dtype == MCKE_DTYPE_BF16) launch_forward(static_cast<const uint16_t*>(logits), a, rows, s);
+  else launch_forward(static_cast<const float*>(logits), a, rows, s);
   return check_launch(who);
 }
 
@@ -227,11 +606,10 @@ extern "C" int mcke_sm100_token_logprobs_backward(const void* logits, int64_t st
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const Grads g = {lse, targets, grad_logprobs, entropy, grad_entropy, grad_lse};
   if (dtype == MCKE_DTYPE_BF16)
-    launch_async(token_logprobs_backward_kernel<uint16_t>, static_cast<unsigned>(rows), kThreads, 0, s,
-                 static_cast<const uint16_t*>(logits), stride, static_cast<uint16_t*>(dlogits), dlogits_stride, cols,
-                 g);
+    MCKE_RETURN_IF(launch_backward(who, static_cast<const uint16_t*>(logits), stride, static_cast<uint16_t*>(dlogits),
+                                   dlogits_stride, rows, cols, g, s));
   else
-    launch_async(token_logprobs_backward_kernel<float>, static_cast<unsigned>(rows), kThreads, 0, s,
-                 static_cast<const float*>(logits), stride, static_cast<float*>(dlogits), dlogits_stride, cols, g);
+    MCKE_RETURN_IF(launch_backward(who, static_cast<const float*>(logits), stride, static_cast<float*>(dlogits),
+                                   dlogits_stride, rows, cols, g, s));
   return check_launch(who);
 }
