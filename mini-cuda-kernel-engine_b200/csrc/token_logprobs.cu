@@ -14,6 +14,8 @@
 // no gradient.  A NaN or +inf in a row makes its results NaN.  A negative
 // target is padding (lp = 0, no gradient through lp); a target past the last
 // column gives NaN and reads nothing.
+#include <type_traits>
+
 #include "row_ops.cuh"
 
 namespace mcke_sm100 {
@@ -99,32 +101,39 @@ __device__ __forceinline__ float exp2_fast(float t) {
   return r;
 }
 
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float r;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Running statistics of a part of a row: its maximum m, s = sum 2^t and
-// w = sum 2^t t with t = (x - m) log2 e.  Where there is nothing but -inf,
-// m = -inf and s = w = 0.
+// w = sum 2^t t with t = (x - m) log2 e, so that the maximum itself counts exactly
+// 1 and 0.  Where there is nothing but -inf, m = -inf and s = w = 0.
 struct Stats {
   float m, s, w;
 };
 // What a maximum of -inf is replaced by, so that x - m is -inf and not NaN.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
-// The sums of `a` on the scale of a maximum m (>= a.m, finite_max applied).
+// The sums of `a` on the scale of a maximum m >= a.m.
 __device__ __forceinline__ Stats rescale(const Stats& a, float m) {
-  const float t = a.m == -INFINITY ? 0.0f : (a.m - m) * kLog2E;
+  if (m == a.m || a.m == -INFINITY) return Stats{m, a.s, a.w};
+  const float t = (a.m - m) * kLog2E;
   const float f = exp2_fast(t);
   // a maximum so far above that nothing is left: f = 0, and t may be -inf
   return Stats{m, a.s * f, f == 0.0f ? 0.0f : f * fmaf(a.s, t, a.w)};
 }
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   const float m = max_nan(a.m, b.m);
-  const Stats p = rescale(a, finite_max(m)), q = rescale(b, finite_max(m));
+  const Stats p = rescale(a, m), q = rescale(b, m);
   return Stats{m, p.s + q.s, p.w + q.w};
 }
 
 // Order of the alternatives: larger value first (NaN above all, -0 equal to
-// +0), then lower index.  Never 0, so 0 stands for "none".
+// +0), then lower index.  Never 0, which stands for "none", nor all ones.
 __device__ __forceinline__ uint32_t order_key(float v) {
   const uint32_t u = __float_as_uint(v + 0.0f);
-  return (v != v) ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return (v != v) ? 0xfffffffeu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
@@ -174,187 +183,298 @@ __device__ __forceinline__ void cluster_barrier() {
 
 constexpr int kMaxCluster = 8;
 constexpr int kLoads = 4;  // vectors of a thread in flight
+template <class T>
+constexpr int64_t kWarpCols = 32 * kLoads * 4 * Vec<T>::kPer;
 
-// The k likeliest of a block's part of the row, into best[0 .. k) in order.
+// For the entropy 2^t t has to stay finite.  Next to a maximum in (kMaxAbove, kMaxBelow)
+// it is enough to raise the elements below kLow (-inf among them) to it, two bf16 at a
+// time: 2^t is 0 for them, and t = (kLow - m) log2 e is finite.  Otherwise t itself
+// is kept from falling below -200, long after 2^t is 0.
+constexpr float kLow = -5e37f, kMaxAbove = -1e37f, kMaxBelow = 1e38f;
+__device__ __forceinline__ void raise_low(uint4& q, const float*) {
+  q.x = __float_as_uint(max_nan(__uint_as_float(q.x), kLow));
+  q.y = __float_as_uint(max_nan(__uint_as_float(q.y), kLow));
+  q.z = __float_as_uint(max_nan(__uint_as_float(q.z), kLow));
+  q.w = __float_as_uint(max_nan(__uint_as_float(q.w), kLow));
+}
+__device__ __forceinline__ void raise_low(uint4& q, const uint16_t*) {
+  constexpr uint32_t kLowPair = 0xfe16fe16u;  // -4.98e37 twice
+  q.x = max_nan_bf16x2(q.x, kLowPair);
+  q.y = max_nan_bf16x2(q.y, kLowPair);
+  q.z = max_nan_bf16x2(q.z, kLowPair);
+  q.w = max_nan_bf16x2(q.w, kLowPair);
+}
+
+// The k largest of n <= kThreads keys in shared memory (0: none; the others all
+// different), into best[0 .. k) in order, zeros behind them: each thread counts the
+// keys above its own.  By the `threads` threads of a row; `sync` is their barrier.
+template <class Sync>
+__device__ __forceinline__ void k_largest(const uint64_t* keys, int n, uint64_t* best, int k, int t, int threads,
+                                          Sync&& sync) {
+  if (t < k) best[t] = 0;
+  sync();
+  for (int i = t; i < n; i += threads) {
+    const uint64_t mine = keys[i];
+    int above = 0;
+#pragma unroll 8
+    for (int j = 0; j < n; ++j) above += keys[j] > mine;
+    if (mine != 0 && above < k) best[above] = mine;
+  }
+  sync();
+}
+
+// Shared memory of one row's search for its likeliest elements.
+template <int kRowWarps>
+struct TopSpace {
+  uint64_t keys[kRowWarps * MCKE_TOP_MAX];  // the warps' lists, k entries each
+  uint64_t best[MCKE_TOP_MAX];
+};
+
+// The k likeliest of a block's part of the row, into space.best in order.
 //
 // Every warp load is a chunk of 32 vectors whose maximum the first pass left in
-// chunk_max (a 32-bit order key; chunk c of the part is entry c).  Ordered by
-// maximum and, among equals, by position, the k best chunks hold the k best
-// elements: an element of any other chunk has the k chunks' maxima before it.
-// So one warp picks those chunks, and only they are read again; elements below
-// the k-th chunk's maximum are passed over, and each warp keeps its k best in its
-// lanes, in order.
-template <class T>
-__device__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift, uint32_t* chunk_max, int chunks,
-                            int k, uint64_t (*lists)[MCKE_TOP_MAX], int* picked, uint64_t* best) {
+// chunk_max (chunk c of the part is entry c).  Ordered by maximum and, among
+// equals, by position, the k best chunks hold the k best elements: an element of
+// any other chunk has the k chunks' maxima before it.  So each warp picks the k
+// best of its share of the chunks, those lists are joined, and only the chunks
+// picked are read again; elements below the k-th chunk's maximum are passed
+// over, and each warp keeps its k best in its lanes, in order.
+template <class T, int kRowWarps, class Sync>
+__device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift,
+                                            const float* chunk_max, int chunks, int k, TopSpace<kRowWarps>& space,
+                                            Sync&& sync) {
   constexpr int kPer = Vec<T>::kPer;
-  __shared__ uint32_t threshold;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int n = k < chunks ? k : chunks;
-  if (warp == 0) {
-    uint32_t last = 0;
-    for (int i = 0; i < n; ++i) {
-      uint64_t key = 0;
-      for (int c = lane; c < chunks; c += 32) {
-        const uint64_t e = (static_cast<uint64_t>(chunk_max[c]) << 32) | static_cast<uint32_t>(~c);
-        if (chunk_max[c] != 0u && e > key) key = e;
-      }
-      key = warp_max_key(key);
-      last = static_cast<uint32_t>(key >> 32);
-      const int c = static_cast<int>(~static_cast<uint32_t>(key));
-      if (lane == 0) {
-        picked[i] = c;
-        chunk_max[c] = 0u;
-      }
-      __syncwarp();
-    }
-    if (lane == 0) threshold = n < k ? 1u : last;  // fewer chunks than k: all of their elements count
-  }
-  __syncthreads();
-  uint64_t mine = 0;  // lane l: this warp's l-th best
-  for (int i = warp; i < n; i += kWarps) {
-    const int64_t first = (first_vec + static_cast<int64_t>(picked[i]) * 32 + lane) * kPer - shift;
-    const uint4 q = ld_row(row, first, cols);
-    F2 v[kPer / 2];
-    unpack(q, v, row);
+  constexpr int kHeld = 2;  // chunk maxima of a lane that stay in registers
+  const int lane = threadIdx.x & 31, warp = kRowWarps == 1 ? 0 : threadIdx.x >> 5;
+  const int t = kRowWarps == 1 ? lane : threadIdx.x;
+  {
+    // this warp's share of the chunks: c = warp + kRowWarps * (lane + 32 i)
+    const int share = (chunks - warp + kRowWarps - 1) / kRowWarps;
+    auto key_of = [&](int i) -> uint64_t {
+      const int at = lane + 32 * i, c = warp + kRowWarps * at;
+      return at < share ? (static_cast<uint64_t>(order_key(chunk_max[c])) << 32) | static_cast<uint32_t>(~c) : 0;
+    };
+    uint64_t held[kHeld];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const float x = j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x;
-      const uint32_t value = order_key(x);
-      const bool in_row = first + j >= 0 && first + j < cols;
-      unsigned todo = __ballot_sync(0xffffffffu, in_row && value >= threshold);
-      while (todo) {
-        const int from = __ffs(todo) - 1;
-        todo &= todo - 1;
-        const uint64_t key = (static_cast<uint64_t>(__shfl_sync(0xffffffffu, value, from)) << 32) |
-                             static_cast<uint32_t>(~static_cast<uint32_t>(first + j + (from - lane) * kPer));
-        const int at = __popc(__ballot_sync(0xffffffffu, mine > key));
-        const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
-        if (lane == at) mine = key;
-        else if (lane > at) mine = up;
+    for (int i = 0; i < kHeld; ++i) held[i] = key_of(i);
+    uint64_t last = ~uint64_t{0};
+    for (int i = 0; i < k; ++i) {
+      uint64_t key = 0;
+      if (i < share) {
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h)
+          if (held[h] < last && held[h] > key) key = held[h];
+        for (int h = kHeld; 32 * h < share; ++h) {
+          const uint64_t e = key_of(h);
+          if (e < last && e > key) key = e;
+        }
+        key = warp_max_key(key);
+        last = key;
+      }
+      if (lane == 0) space.keys[warp * k + i] = key;
+    }
+  }
+  sync();
+  const uint64_t* picked = space.keys;
+  if constexpr (kRowWarps > 1) {
+    k_largest(space.keys, kRowWarps * k, space.best, k, t, 32 * kRowWarps, sync);
+    picked = space.best;
+  }
+  // fewer chunks than k: all of their elements count
+  const int n = k < chunks ? k : chunks;
+  const float threshold = n < k ? -INFINITY : key_value(static_cast<uint32_t>(picked[k - 1] >> 32));
+  constexpr int kBatch = 2;  // chunks of a warp in flight
+  uint64_t mine = 0;         // lane l: this warp's l-th best
+  for (int i0 = warp; i0 < n; i0 += kRowWarps * kBatch) {
+    uint4 q[kBatch];
+    int64_t first[kBatch];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * kRowWarps;
+      if (i >= n) break;
+      const int c = static_cast<int>(~static_cast<uint32_t>(picked[i]));
+      first[u] = (first_vec + static_cast<int64_t>(c) * 32 + lane) * kPer - shift;
+      q[u] = ld_row(row, first[u], cols);
+    }
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      if (i0 + u * kRowWarps >= n) break;
+      // elements lo .. hi of the vector are the row's
+      const int lo = static_cast<int>(max(-first[u], int64_t{0}));
+      const int hi = static_cast<int>(min(cols - first[u], static_cast<int64_t>(kPer)));
+      F2 v[kPer / 2];
+      unpack(q[u], v, row);
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const float x = j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x;
+        // not below: a NaN is above all
+        unsigned todo = __ballot_sync(0xffffffffu, !(x < threshold) && j >= lo && j < hi);
+        while (todo) {
+          const int from = __ffs(todo) - 1;
+          todo &= todo - 1;
+          const uint64_t key = (static_cast<uint64_t>(order_key(__shfl_sync(0xffffffffu, x, from))) << 32) |
+                               static_cast<uint32_t>(~static_cast<uint32_t>(first[u] + j + (from - lane) * kPer));
+          const int at = __popc(__ballot_sync(0xffffffffu, mine > key));
+          const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
+          if (lane == at) mine = key;
+          else if (lane > at) mine = up;
+        }
       }
     }
   }
-  if (lane < k) lists[warp][lane] = mine;
-  __syncthreads();
-  if (warp == 0) {  // lane w walks warp w's list
-    int at = 0;
-    for (int i = 0; i < k; ++i) {
-      const uint64_t head = lane < kWarps && at < k ? lists[lane][at] : 0;
-      const uint64_t key = warp_max_key(head);
-      if (head == key && key != 0) ++at;
-      if (lane == 0) best[i] = key;
-    }
+  sync();  // everybody has read what was picked
+  if constexpr (kRowWarps > 1) {
+    if (lane < k) space.keys[warp * k + lane] = mine;
+    sync();
+    k_largest(space.keys, kRowWarps * k, space.best, k, t, 32 * kRowWarps, sync);
+  } else {
+    if (lane < k) space.best[lane] = mine;
+    sync();
   }
 }
 
-// A row to each cluster of 1, 2, 4 or 8 blocks, each with a run of the row's chunks:
-// one read of the row with a running maximum and the two sums on its scale; the
-// blocks' results are joined in the first block's shared memory, in order.
-template <class T, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __restrict__ x, const ForwardArgs a) {
+// kRowWarps = kWarps: a row to each cluster of 1, 2, 4 or 8 blocks, each block with a run
+// of the row's chunks; the blocks' results are joined in the first block's
+// shared memory, in order.  kRowWarps = 1: a row to each warp, eight to a block.
+//
+// One read of the row: a warp has kLoads chunks in flight, takes their maximum, and
+// adds up the sums on its scale.
+template <class T, int kRowWarps, bool kEntropy, bool kTop>
+__global__ void __launch_bounds__(kThreads)
+    token_logprobs_kernel(const T* __restrict__ x, const ForwardArgs a, int64_t rows, int max_chunks) {
   pdl_entry();
   constexpr int kPer = Vec<T>::kPer, kPairs = kPer / 2;
-  extern __shared__ uint32_t chunk_max[];
+  constexpr int kRows = kWarps / kRowWarps;
+  extern __shared__ float chunk_maxima[];  // [kRows][max_chunks]
   __shared__ Stats warp_stats[kWarps];
-  __shared__ Stats part_stats[kMaxCluster];
-  __shared__ uint64_t part_best[kTop ? kMaxCluster : 1][MCKE_TOP_MAX];
-  __shared__ uint64_t lists[kTop ? kWarps : 1][MCKE_TOP_MAX];
-  __shared__ int picked[MCKE_TOP_MAX];
-  const uint32_t blocks = cluster_blocks(), block = cluster_block();
-  const int64_t row = blockIdx.x / blocks;
+  __shared__ Stats part_stats[kRowWarps == 1 ? 1 : kMaxCluster];
+  __shared__ uint64_t part_best[kTop && kRowWarps > 1 ? kMaxCluster * MCKE_TOP_MAX : 1];
+  __shared__ TopSpace<kRowWarps> top_space[kTop ? kRows : 1];
+  const int lane = threadIdx.x & 31, warp = kRowWarps == 1 ? 0 : threadIdx.x >> 5;
+  const int slot = kRowWarps == 1 ? threadIdx.x >> 5 : 0;
+  const uint32_t blocks = kRowWarps == 1 ? 1 : cluster_blocks(), block = kRowWarps == 1 ? 0 : cluster_block();
+  const int64_t row = kRowWarps == 1 ? static_cast<int64_t>(blockIdx.x) * kRows + slot : blockIdx.x / blocks;
+  if (kRowWarps == 1 && row >= rows) return;
+  auto sync = [] {
+    if constexpr (kRowWarps == 1) __syncwarp();
+    else __syncthreads();
+  };
+  float* const chunk_max = chunk_maxima + slot * max_chunks;
   const T* xr = x + row * a.stride;
   const int shift = vec_shift(xr);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t vecs = (a.cols + shift + kPer - 1) / kPer;
   const int64_t all_chunks = (vecs + 31) / 32;
   const int64_t chunk0 = all_chunks * block / blocks, chunk1 = all_chunks * (block + 1) / blocks;
   const int chunks = static_cast<int>(chunk1 - chunk0);
 
-  Stats st{-INFINITY, 0.0f, 0.0f};
-  for (int c = warp; c < chunks; c += kWarps * kLoads) {
+  // chunks inner0 .. inner1 of the part hold no vector that the row's ends cut
+  const int inner0 = chunk0 == 0 && shift > 0 ? 1 : 0;
+  const int inner1 = static_cast<int>(min((a.cols + shift) / (32 * kPer), chunk1) - chunk0);
+  const T* const inner = xr + (chunk0 * 32 + lane) * kPer - shift;
+
+  Stats st{-INFINITY, 0.0f, 0.0f};  // m is the warp's, the sums are the lane's
+  for (int c = warp; c < chunks; c += kRowWarps * kLoads) {
     uint4 q[kLoads];
+    if (c >= inner0 && c + (kLoads - 1) * kRowWarps < inner1) {
+      const T* p = inner + static_cast<int64_t>(c) * (32 * kPer);
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const int64_t v = (chunk0 + c + u * kWarps) * 32 + lane;
-      q[u] = c + u * kWarps < chunks ? ld_row(xr, v * kPer - shift, a.cols)
-                                     : ld_row(xr, a.cols, a.cols);  // past the row: -inf
-    }
-    float m = st.m;
+      for (int u = 0; u < kLoads; ++u) q[u] = ld_vec(p + u * kRowWarps * (32 * kPer));
+    } else {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      const float mu = vec_max(q[u], xr);
-      if constexpr (kTop) {
-        const uint32_t key = __reduce_max_sync(0xffffffffu, order_key(mu));
-        if (lane == 0 && c + u * kWarps < chunks) chunk_max[c + u * kWarps] = key;
+      for (int u = 0; u < kLoads; ++u) {
+        const int64_t v = (chunk0 + c + u * kRowWarps) * 32 + lane;
+        const int64_t first = c + u * kRowWarps < chunks ? v * kPer - shift : a.cols;  // past the row: -inf
+        q[u] = ld_row(xr, first, a.cols);
       }
-      m = max_nan(m, mu);
     }
-    const float mf = finite_max(m);
-    st = rescale(st, mf);
-    st.m = m;
-    const F2 minus_m = f2(-mf), scale = f2(kLog2E);
+    float m;
+    if constexpr (kTop) {
+      m = st.m;
+#pragma unroll
+      for (int u = 0; u < kLoads; ++u) {
+        const float mu = warp_max_nan(vec_max(q[u], xr));
+        if (lane == 0 && c + u * kRowWarps < chunks) chunk_max[c + u * kRowWarps] = mu;
+        m = max_nan(m, mu);
+      }
+    } else {
+      m = vec_max(q[0], xr);
+#pragma unroll
+      for (int u = 1; u < kLoads; ++u) m = max_nan(m, vec_max(q[u], xr));
+      m = max_nan(st.m, warp_max_nan(m));
+    }
+    st = rescale(st, m);
     F2 s2 = f2(0.0f), w2 = f2(0.0f);
+    const F2 scale = f2(kLog2E), minus_m = f2(-finite_max(m));
+    auto add_up = [&](auto raise) {
 #pragma unroll
-    for (int u = 0; u < kLoads; ++u) {
-      F2 v[kPairs];
-      unpack(q[u], v, xr);
+      for (int u = 0; u < kLoads; ++u) {
+        if constexpr (kEntropy && decltype(raise)::value) raise_low(q[u], xr);
+        F2 v[kPairs];
+        unpack(q[u], v, xr);
 #pragma unroll
-      for (int j = 0; j < kPairs; ++j) {
-        float2 t = split(mul2(add2(v[j], minus_m), scale));
-        if constexpr (kEntropy) {
-          // 2^t is 0 long before -200; t itself has to stay finite for 2^t t
-          t.x = max_nan(t.x, -200.0f);
-          t.y = max_nan(t.y, -200.0f);
+        for (int j = 0; j < kPairs; ++j) {
+          F2 tt = mul2(add2(v[j], minus_m), scale);
+          float2 t = split(tt);
+          if constexpr (kEntropy && !decltype(raise)::value) {
+            t.x = max_nan(t.x, -200.0f);
+            t.y = max_nan(t.y, -200.0f);
+            tt = f2(t.x, t.y);
+          }
+          const F2 e = f2(exp2_fast(t.x), exp2_fast(t.y));
+          s2 = add2(s2, e);
+          if constexpr (kEntropy) w2 = fma2(e, tt, w2);
         }
-        const F2 e = f2(exp2_fast(t.x), exp2_fast(t.y));
-        s2 = add2(s2, e);
-        if constexpr (kEntropy) w2 = fma2(e, f2(t.x, t.y), w2);
       }
-    }
+    };
+    if (!kEntropy || (m > kMaxAbove && m < kMaxBelow)) add_up(std::true_type{});
+    else add_up(std::false_type{});
     st.s += sum2(s2);
     if constexpr (kEntropy) st.w += sum2(w2);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats other;
-    other.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    other.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    other.w = kEntropy ? __shfl_xor_sync(0xffffffffu, st.w, o) : 0.0f;
-    st = join(st, other);
+  st.s = warp_all_sum(st.s);
+  if constexpr (kEntropy) st.w = warp_all_sum(st.w);
+  if constexpr (kRowWarps > 1) {
+    if (lane == 0) warp_stats[warp] = st;
   }
-  if (lane == 0) warp_stats[warp] = st;
-  __syncthreads();
+  sync();
   if constexpr (kTop)
-    top_of_part(xr, a.cols, chunk0 * 32, shift, chunk_max, chunks, a.top_k, lists, picked, part_best[block]);
-  if (threadIdx.x == 0) {
-    st = warp_stats[0];
+    top_of_part<T, kRowWarps>(xr, a.cols, chunk0 * 32, shift, chunk_max, chunks, a.top_k, top_space[slot], sync);
+  const uint64_t* best = top_space[slot].best;
+  if constexpr (kRowWarps > 1) {
+    // the warps' statistics, a lane to each: the same bits in every lane
+    auto join_lanes = [&](Stats s8) {
 #pragma unroll
-    for (int w = 1; w < kWarps; ++w) st = join(st, warp_stats[w]);
-    part_stats[block] = st;
-  }
-  if (blocks > 1) {
-    __syncthreads();
-    cluster_barrier();  // every block of the cluster runs: its shared memory may be written
-    if (block > 0) {
-      const uint32_t to = address_in_block(&part_stats[block], 0);
-      const uint32_t words[3] = {__float_as_uint(part_stats[block].m), __float_as_uint(part_stats[block].s),
-                                 __float_as_uint(part_stats[block].w)};
-      if (threadIdx.x < 3)
-        asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * threadIdx.x), "r"(words[threadIdx.x]) : "memory");
-      if (kTop && threadIdx.x < a.top_k)
-        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(address_in_block(&part_best[block][threadIdx.x], 0)),
-                     "l"(part_best[block][threadIdx.x])
+      for (int o = 4; o > 0; o >>= 1)
+        s8 = join(s8, Stats{__shfl_xor_sync(0xffffffffu, s8.m, o), __shfl_xor_sync(0xffffffffu, s8.s, o),
+                            __shfl_xor_sync(0xffffffffu, s8.w, o)});
+      return s8;
+    };
+    static_assert(kWarps == 8 && kMaxCluster == 8, "eight lanes");
+    if (warp == 0) st = join_lanes(warp_stats[lane & 7]);
+    if (blocks > 1) {
+      cluster_barrier();  // every block of the cluster runs: its shared memory may be written
+      if (threadIdx.x < 3) {
+        const float v = threadIdx.x == 0 ? st.m : threadIdx.x == 1 ? st.s : st.w;
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address_in_block(&part_stats[block], 0) + 4 * threadIdx.x),
+                     "f"(v)
                      : "memory");
+      }
+      if (kTop && threadIdx.x < a.top_k)
+        asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(
+                         address_in_block(&part_best[block * a.top_k + threadIdx.x], 0)),
+                     "l"(best[threadIdx.x])
+                     : "memory");
+      cluster_barrier();
+      if (block > 0) return;
+      if constexpr (kTop)
+        k_largest(part_best, static_cast<int>(blocks) * a.top_k, top_space[slot].best, a.top_k, threadIdx.x, kThreads,
+                  sync);
     }
-    cluster_barrier();
-    if (block > 0) return;
+    if (warp > 0) return;
+    if (blocks > 1)
+      st = join_lanes((lane & 7) < static_cast<int>(blocks) ? part_stats[lane & 7] : Stats{-INFINITY, 0.0f, 0.0f});
   }
-  if (warp > 0) return;
-  __syncwarp();
-  st = part_stats[0];
-  for (uint32_t b = 1; b < blocks; ++b) st = join(st, part_stats[b]);
-  // a row of which nothing is left (a NaN or +inf makes s NaN: it has no such row)
+  // a row of which nothing is left (with a NaN or +inf in it, m or s is not so)
   const bool none = st.m == -INFINITY;
   const float ln_s = logf(st.s);
   auto logprob = [&](float v) { return none ? -INFINITY : (v - st.m) - ln_s; };
@@ -366,18 +486,9 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_kernel(const T* __res
       a.logprobs[row] = t < 0 ? 0.0f : t >= a.cols ? NAN : logprob(ld_val(xr + t));
     }
   }
-  if constexpr (kTop) {
-    // lane b walks block b's list
-    int at = 0;
-    for (int i = 0; i < a.top_k; ++i) {
-      const uint64_t head = lane < static_cast<int>(blocks) && at < a.top_k ? part_best[lane][at] : 0;
-      const uint64_t key = warp_max_key(head);
-      if (head == key && key != 0) ++at;
-      if (lane == 0) {
-        a.top_ids[row * a.top_k + i] = key_index(key);
-        a.top_logprobs[row * a.top_k + i] = logprob(key_value(static_cast<uint32_t>(key >> 32)));
-      }
-    }
+  if (kTop && lane < a.top_k) {
+    a.top_ids[row * a.top_k + lane] = key_index(best[lane]);
+    a.top_logprobs[row * a.top_k + lane] = logprob(key_value(static_cast<uint32_t>(best[lane] >> 32)));
   }
 }
 
@@ -391,17 +502,22 @@ struct Grads {
 };
 
 // dx may be x itself: a vector is read before it is written, by the same thread.
-// A block takes kVecs vectors of a row to a thread; kSame: dx has the row's offset from
-// a 16-byte boundary, so whole vectors are stored.
+// `threads` threads of a block (a power of two) take a part of a row, kVecs vectors
+// each; kSame: dx has the row's offset from a 16-byte boundary, so whole vectors
+// are stored.
 constexpr int kVecs = 4;
 template <class T, bool kEntropy, bool kSame>
-__global__ void __launch_bounds__(kThreads)
-    token_logprobs_backward_kernel(const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t cols, int parts,
-                                   Grads g) {
+__global__ void __launch_bounds__(kThreads, 6)
+    token_logprobs_backward_kernel(const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t rows, int64_t cols,
+                                   int parts, int threads, Grads g) {
   pdl_entry();
   constexpr int kPer = Vec<T>::kPer, kPairs = kPer / 2;
-  const int64_t row = blockIdx.x / parts;
-  const int64_t part = blockIdx.x - row * parts;
+  const int t0 = threadIdx.x & (threads - 1);
+  // a block to a part of a row, or (parts == 1) several rows to a block
+  const int64_t row = parts > 1 ? blockIdx.x / static_cast<unsigned>(parts)
+                                : static_cast<int64_t>(blockIdx.x) * (kThreads / threads) + threadIdx.x / threads;
+  const int part = parts > 1 ? static_cast<int>(blockIdx.x % static_cast<unsigned>(parts)) : 0;
+  if (row >= rows) return;
   const T* xr = x + row * stride;
   T* dxr = dx + row * dx_stride;
   const int shift = vec_shift(xr);
@@ -409,8 +525,8 @@ __global__ void __launch_bounds__(kThreads)
   uint4 q[kVecs];
 #pragma unroll
   for (int u = 0; u < kVecs; ++u) {
-    first[u] = ((part * kVecs + u) * kThreads + threadIdx.x) * kPer - shift;
-    q[u] = ld_row(xr, first[u] < cols ? first[u] : cols, cols);
+    first[u] = (static_cast<int64_t>(part * kVecs + u) * threads + t0) * kPer - shift;
+    q[u] = ld_row(xr, min(first[u], cols), cols);
   }
   const float lse = g.lse[row];
   const int64_t t = g.logprobs ? g.targets[row] : -1;
@@ -481,22 +597,31 @@ int row_blocks(int64_t rows, int64_t cols) {
   while (n < kMaxCluster && 2 * n * rows <= 2 * 148 && n < rounds) n *= 2;
   return n;
 }
-
+// A row to a warp where a block would have less than a round of loads for it and there
+// are rows enough for every SM's warps.
 template <class T>
+bool warp_rows(int64_t rows, int64_t cols) {
+  return cols <= kWarpCols<T> && rows >= 148 * kWarps;
+}
+
+template <class T, int kRowWarps>
 void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
-  const int blocks = row_blocks<T>(rows, a.cols);
+  const int blocks = kRowWarps == 1 ? 1 : row_blocks<T>(rows, a.cols);
   const bool top = a.top_k > 0;
-  // the largest part's chunk maxima
+  // the chunk maxima of the largest part, whatever the row's shift
   const int64_t chunks = ((a.cols + Vec<T>::kPer - 1) / Vec<T>::kPer + 1 + 31) / 32;
-  const std::size_t smem = top ? static_cast<std::size_t>((chunks + blocks - 1) / blocks + 1) * 4 : 0;
-  auto kernel = a.entropy ? (top ? token_logprobs_kernel<T, true, true> : token_logprobs_kernel<T, true, false>)
-                          : (top ? token_logprobs_kernel<T, false, true> : token_logprobs_kernel<T, false, false>);
+  const int max_chunks = top ? static_cast<int>((chunks + blocks - 1) / blocks + 1) : 0;
+  const std::size_t smem = static_cast<std::size_t>(max_chunks) * (kWarps / kRowWarps) * sizeof(float);
+  auto kernel = a.entropy ? (top ? token_logprobs_kernel<T, kRowWarps, true, true>
+                                 : token_logprobs_kernel<T, kRowWarps, true, false>)
+                          : (top ? token_logprobs_kernel<T, kRowWarps, false, true>
+                                 : token_logprobs_kernel<T, kRowWarps, false, false>);
   if (smem > 32 * 1024)
     cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(smem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(static_cast<unsigned>(rows * blocks));
+  cfg.gridDim = dim3(static_cast<unsigned>(kRowWarps == 1 ? (rows + kWarps - 1) / kWarps : rows * blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
@@ -511,24 +636,33 @@ void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
   }
-  cudaLaunchKernelEx(&cfg, kernel, x, a);  // errors are left for check_launch()
+  cudaLaunchKernelEx(&cfg, kernel, x, a, rows, max_chunks);  // errors are left for check_launch()
+}
+
+template <class T>
+void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
+  if (warp_rows<T>(rows, a.cols)) launch_forward<T, 1>(x, a, rows, s);
+  else launch_forward<T, kWarps>(x, a, rows, s);
 }
 
 template <class T>
 int launch_backward(const char* who, const T* x, int64_t stride, T* dx, int64_t dx_stride, int64_t rows, int64_t cols,
                     const Grads& g, cudaStream_t s) {
   constexpr int kPer = Vec<T>::kPer;
-  const int64_t per_block = static_cast<int64_t>(kThreads) * kVecs * kPer;
-  const int64_t parts = (cols + kPer - 1 + per_block - 1) / per_block;  // whatever the row's shift
-  if (rows * parts > 2147483647LL) return fail(MCKE_INVALID_ARGUMENT, "%s: too many elements for one launch", who);
+  const int64_t vecs = (cols + kPer - 1 + kPer - 1) / kPer;  // whatever the row's shift
+  int threads = 32;
+  while (threads < kThreads && threads * kVecs < vecs) threads *= 2;
+  const int64_t parts = (vecs + threads * kVecs - 1) / (threads * kVecs);
+  const int64_t blocks = (rows * parts + kThreads / threads - 1) / (kThreads / threads);
+  if (blocks > 2147483647LL) return fail(MCKE_INVALID_ARGUMENT, "%s: too many elements for one launch", who);
   const bool same = (reinterpret_cast<std::uintptr_t>(x) - reinterpret_cast<std::uintptr_t>(dx)) % 16 == 0 &&
                     (rows == 1 || (stride - dx_stride) % kPer == 0);
   auto kernel = g.grad_entropy ? (same ? token_logprobs_backward_kernel<T, true, true>
                                        : token_logprobs_backward_kernel<T, true, false>)
                                : (same ? token_logprobs_backward_kernel<T, false, true>
                                        : token_logprobs_backward_kernel<T, false, false>);
-  launch_async(kernel, static_cast<unsigned>(rows * parts), kThreads, 0, s, x, stride, dx, dx_stride, cols,
-               static_cast<int>(parts), g);
+  launch_async(kernel, static_cast<unsigned>(blocks), kThreads, 0, s, x, stride, dx, dx_stride, rows, cols,
+               static_cast<int>(parts), threads, g);
   return MCKE_OK;
 }
 
