@@ -21,8 +21,7 @@
 namespace mcke_sm100 {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kWarps = kThreads / 32;
+constexpr int kThreads = 256;    // of the backward pass
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -138,15 +137,23 @@ __device__ __forceinline__ uint32_t order_key(float v) {
 __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
 }
+__device__ __forceinline__ uint64_t full_key(float v, uint32_t index) {
+  return (static_cast<uint64_t>(order_key(v)) << 32) | static_cast<uint32_t>(~index);
+}
 __device__ __forceinline__ int64_t key_index(uint64_t key) {
   return static_cast<uint32_t>(~static_cast<uint32_t>(key));
 }
-// The largest of the warp's 64-bit keys.
-__device__ __forceinline__ uint64_t warp_max_key(uint64_t v) {
-  const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32));
-  const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(v >> 32) == hi ? static_cast<uint32_t>(v) : 0u);
-  return (static_cast<uint64_t>(hi) << 32) | lo;
-}
+// Dynamic shared memory of one row's search, in 8-byte words (an even number): the keys
+// of the chunks of MCKE_TOP_MAX runs, where a run is more than one chunk, and the
+// maxima of max_chunks chunks.
+struct TopScratch {
+  int run_keys, words;
+  __host__ __device__ TopScratch(int max_chunks, int threads) {
+    const int run = (max_chunks + threads - 1) / threads;
+    run_keys = run > 1 ? MCKE_TOP_MAX * run : 0;
+    words = run_keys + (max_chunks + 3) / 4 * 2;
+  }
+};
 
 struct ForwardArgs {
   int64_t stride, cols;
@@ -205,151 +212,208 @@ __device__ __forceinline__ void raise_low(uint4& q, const uint16_t*) {
   q.w = max_nan_bf16x2(q.w, kLowPair);
 }
 
-// The k largest of n <= kThreads keys in shared memory (0: none; the others all
-// different), into best[0 .. k) in order, zeros behind them: each thread counts the
-// keys above its own.  By the `threads` threads of a row; `sync` is their barrier.
+// Shared memory of one row's search for its likeliest elements.
+template <int kRowWarps>
+struct TopSpace {
+  static constexpr int kThreads = 32 * kRowWarps;
+  alignas(16) uint64_t keys[kThreads];  // a key to each of the row's threads
+  alignas(16) uint64_t best[MCKE_TOP_MAX];
+  int count[kRowWarps];                 // of each warp's 32 keys, those in use
+};
+
+// The k largest of n different keys in shared memory, into best[0 .. k) in order, zeros
+// behind them if there are fewer: each thread counts the keys above its own.  keys
+// is 16-byte aligned, and keys[n] = 0 where n is odd.  By the `threads` threads of a
+// row; `sync` is their barrier.
 template <class Sync>
 __device__ __forceinline__ void k_largest(const uint64_t* keys, int n, uint64_t* best, int k, int t, int threads,
                                           Sync&& sync) {
   if (t < k) best[t] = 0;
   sync();
+  const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(keys);
   for (int i = t; i < n; i += threads) {
     const uint64_t mine = keys[i];
     int above = 0;
 #pragma unroll 8
-    for (int j = 0; j < n; ++j) above += keys[j] > mine;
-    if (mine != 0 && above < k) best[above] = mine;
+    for (int j = 0; 2 * j < n; ++j) {
+      const ulonglong2 p = pairs[j];
+      above += (p.x > mine) + (p.y > mine);
+    }
+    if (above < k) best[above] = mine;
   }
   sync();
 }
 
-// Shared memory of one row's search for its likeliest elements.
-template <int kRowWarps>
-struct TopSpace {
-  uint64_t keys[kRowWarps * MCKE_TOP_MAX];  // the warps' lists, k entries each
-  uint64_t best[MCKE_TOP_MAX];
-};
+// One warp's choice of the k largest chunk maxima, one after the other, into best: for
+// small k cheaper than counting ranks, though the other warps wait for it (8192 x 32768
+// bf16, k = 5: 118 us against 129; 1024 x 131072, k = 20: 82 us against 68).  A row
+// that has one warp counts in any case (8192 x 2000 f32, k = 8: 26.6 us against 24.6).
+constexpr int kFewTop = 8;
+__device__ __forceinline__ void pick_chunks(const float* chunk_max, int chunks, int k, uint64_t* best) {
+  constexpr int kHeld = 4;  // keys of a lane that stay in registers
+  const int lane = threadIdx.x & 31;
+  auto key_of = [&](int i) { return lane + 32 * i < chunks ? full_key(chunk_max[lane + 32 * i], lane + 32 * i) : 0; };
+  uint64_t held[kHeld];
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) held[i] = key_of(i);
+  uint64_t last = ~uint64_t{0};
+  for (int i = 0; i < k && i < chunks; ++i) {
+    uint64_t key = 0;
+#pragma unroll
+    for (int h = 0; h < kHeld; ++h)
+      if (held[h] < last && held[h] > key) key = held[h];
+    for (int h = kHeld; 32 * h < chunks; ++h) {
+      const uint64_t e = key_of(h);
+      if (e < last && e > key) key = e;
+    }
+    const uint32_t hi = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32));
+    const uint32_t lo = __reduce_max_sync(0xffffffffu, static_cast<uint32_t>(key >> 32) == hi ? static_cast<uint32_t>(key) : 0u);
+    last = (static_cast<uint64_t>(hi) << 32) | lo;
+    if (lane == 0) best[i] = last;
+  }
+}
 
 // The k likeliest of a block's part of the row, into space.best in order.
 //
 // Every warp load is a chunk of 32 vectors whose maximum the first pass left in
 // chunk_max (chunk c of the part is entry c).  Ordered by maximum and, among
 // equals, by position, the k best chunks hold the k best elements: an element of
-// any other chunk has the k chunks' maxima before it.  So each warp picks the k
-// best of its share of the chunks, those lists are joined, and only the chunks
-// picked are read again; elements below the k-th chunk's maximum are passed
-// over, and each warp keeps its k best in its lanes, in order.
+// any other chunk has the k chunks' maxima before it.  In the same way the k best
+// runs of `run` chunks hold the k best chunks; a run to a thread, so that ranks come
+// from counting.  Only the k chunks are read again.  Their elements that the k-th
+// maximum does not rule out, a few more than k, are left in 32 places of their
+// warp and ranked; a warp that equal values give more than that keeps its k best in
+// its lanes instead.
 template <class T, int kRowWarps, class Sync>
 __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift,
-                                            const float* chunk_max, int chunks, int k, TopSpace<kRowWarps>& space,
-                                            Sync&& sync) {
-  constexpr int kPer = Vec<T>::kPer;
-  constexpr int kHeld = 2;  // chunk maxima of a lane that stay in registers
+                                            const float* chunk_max, uint64_t* run_keys, int chunks, int k,
+                                            TopSpace<kRowWarps>& space, Sync&& sync) {
+  constexpr int kPer = Vec<T>::kPer, kThreads = TopSpace<kRowWarps>::kThreads;
+  constexpr int kBatch = 2;  // chunks of a warp in flight
   const int lane = threadIdx.x & 31, warp = kRowWarps == 1 ? 0 : threadIdx.x >> 5;
   const int t = kRowWarps == 1 ? lane : threadIdx.x;
-  {
-    // this warp's share of the chunks: c = warp + kRowWarps * (lane + 32 i)
-    const int share = (chunks - warp + kRowWarps - 1) / kRowWarps;
-    auto key_of = [&](int i) -> uint64_t {
-      const int at = lane + 32 * i, c = warp + kRowWarps * at;
-      return at < share ? (static_cast<uint64_t>(order_key(chunk_max[c])) << 32) | static_cast<uint32_t>(~c) : 0;
-    };
-    uint64_t held[kHeld];
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) held[i] = key_of(i);
-    uint64_t last = ~uint64_t{0};
-    for (int i = 0; i < k; ++i) {
-      uint64_t key = 0;
-      if (i < share) {
-#pragma unroll
-        for (int h = 0; h < kHeld; ++h)
-          if (held[h] < last && held[h] > key) key = held[h];
-        for (int h = kHeld; 32 * h < share; ++h) {
-          const uint64_t e = key_of(h);
-          if (e < last && e > key) key = e;
-        }
-        key = warp_max_key(key);
-        last = key;
+  uint64_t key = 0;
+  if (kRowWarps > 1 && k <= kFewTop) {
+    if (warp == 0) pick_chunks(chunk_max, chunks, k, space.best);
+    sync();
+  } else {
+    const int run = (chunks + kThreads - 1) / kThreads, runs = (chunks + run - 1) / run;
+    for (int c = t * run; c < min((t + 1) * run, chunks); ++c) key = max(key, full_key(chunk_max[c], c));
+    space.keys[t] = key;
+    k_largest(space.keys, runs, space.best, k, t, kThreads, sync);
+    if (run > 1) {
+      // the chunks of those runs
+      const int n = min(k, runs) * run;
+      for (int i = t; i < n + (n & 1); i += kThreads) {
+        const int c = i < n ? static_cast<int>(key_index(space.best[i / run])) / run * run + i % run : chunks;
+        run_keys[i] = c < chunks ? full_key(chunk_max[c], c) : 0;
       }
-      if (lane == 0) space.keys[warp * k + i] = key;
+      sync();
+      k_largest(run_keys, n, space.best, k, t, kThreads, sync);
     }
+  }
+  const int n = min(k, chunks);
+  // fewer chunks than k: all of their elements count
+  const float threshold = n < k ? -INFINITY : key_value(static_cast<uint32_t>(space.best[k - 1] >> 32));
+  // f(lanes whose element counts, the element's value, its index), for this warp's chunks
+  auto for_candidates = [&](auto&& f) {
+    for (int i0 = warp; i0 < n; i0 += kRowWarps * kBatch) {
+      uint4 q[kBatch];
+      int64_t first[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (i0 + u * kRowWarps >= n) break;
+        first[u] = (first_vec + key_index(space.best[i0 + u * kRowWarps]) * 32 + lane) * kPer - shift;
+        q[u] = ld_row(row, first[u], cols);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        if (i0 + u * kRowWarps >= n) break;
+        // elements lo .. hi of the vector are the row's
+        const int lo = static_cast<int>(max(-first[u], int64_t{0}));
+        const int hi = static_cast<int>(min(cols - first[u], static_cast<int64_t>(kPer)));
+        F2 v[kPer / 2];
+        unpack(q[u], v, row);
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const float x = j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x;
+          // not below: a NaN is above all
+          const unsigned lanes = __ballot_sync(0xffffffffu, !(x < threshold) && j >= lo && j < hi);
+          if (lanes) f(lanes, x, static_cast<uint32_t>(first[u] + j));
+        }
+      }
+    }
+  };
+  uint64_t* const mine = space.keys + 32 * warp;
+  int found = 0;
+  for_candidates([&](unsigned lanes, float x, uint32_t index) {
+    const int at = found + __popc(lanes & ((1u << lane) - 1u));
+    if ((lanes >> lane & 1u) && at < 32) mine[at] = full_key(x, index);
+    found += __popc(lanes);
+  });
+  if (found > 32) {
+    uint64_t listed = 0;  // lane l: this warp's l-th best
+    for_candidates([&](unsigned lanes, float x, uint32_t index) {
+      const uint64_t own = full_key(x, index);
+      // of equal values the first come first: most do not reach the list
+      const uint64_t last = __shfl_sync(0xffffffffu, listed, k - 1);
+      unsigned todo = __ballot_sync(0xffffffffu, (lanes >> lane & 1u) && own > last);
+      while (todo) {
+        const int from = __ffs(todo) - 1;
+        todo &= todo - 1;
+        const uint64_t add = __shfl_sync(0xffffffffu, own, from);
+        const int at = __popc(__ballot_sync(0xffffffffu, listed > add));
+        const uint64_t up = __shfl_up_sync(0xffffffffu, listed, 1);
+        if (lane == at) listed = add;
+        else if (lane > at) listed = up;
+      }
+    });
+    mine[lane] = lane < k ? listed : 0;
+    found = k;
+  } else if (lane >= found) {
+    mine[lane] = 0;
+  }
+  if (lane == 0) space.count[warp] = found;
+  sync();
+  if (t < k) space.best[t] = 0;
+  sync();
+  if (lane < found) {
+    key = mine[lane];
+    int above = 0;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) {
+      const ulonglong2* pairs = reinterpret_cast<const ulonglong2*>(space.keys + 32 * w);
+#pragma unroll 4
+      for (int j = 0; 2 * j < space.count[w]; ++j) {
+        const ulonglong2 p = pairs[j];
+        above += (p.x > key) + (p.y > key);
+      }
+    }
+    if (above < k) space.best[above] = key;
   }
   sync();
-  const uint64_t* picked = space.keys;
-  if constexpr (kRowWarps > 1) {
-    k_largest(space.keys, kRowWarps * k, space.best, k, t, 32 * kRowWarps, sync);
-    picked = space.best;
-  }
-  // fewer chunks than k: all of their elements count
-  const int n = k < chunks ? k : chunks;
-  const float threshold = n < k ? -INFINITY : key_value(static_cast<uint32_t>(picked[k - 1] >> 32));
-  constexpr int kBatch = 2;  // chunks of a warp in flight
-  uint64_t mine = 0;         // lane l: this warp's l-th best
-  for (int i0 = warp; i0 < n; i0 += kRowWarps * kBatch) {
-    uint4 q[kBatch];
-    int64_t first[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * kRowWarps;
-      if (i >= n) break;
-      const int c = static_cast<int>(~static_cast<uint32_t>(picked[i]));
-      first[u] = (first_vec + static_cast<int64_t>(c) * 32 + lane) * kPer - shift;
-      q[u] = ld_row(row, first[u], cols);
-    }
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      if (i0 + u * kRowWarps >= n) break;
-      // elements lo .. hi of the vector are the row's
-      const int lo = static_cast<int>(max(-first[u], int64_t{0}));
-      const int hi = static_cast<int>(min(cols - first[u], static_cast<int64_t>(kPer)));
-      F2 v[kPer / 2];
-      unpack(q[u], v, row);
-#pragma unroll
-      for (int j = 0; j < kPer; ++j) {
-        const float x = j % 2 ? split(v[j / 2]).y : split(v[j / 2]).x;
-        // not below: a NaN is above all
-        unsigned todo = __ballot_sync(0xffffffffu, !(x < threshold) && j >= lo && j < hi);
-        while (todo) {
-          const int from = __ffs(todo) - 1;
-          todo &= todo - 1;
-          const uint64_t key = (static_cast<uint64_t>(order_key(__shfl_sync(0xffffffffu, x, from))) << 32) |
-                               static_cast<uint32_t>(~static_cast<uint32_t>(first[u] + j + (from - lane) * kPer));
-          const int at = __popc(__ballot_sync(0xffffffffu, mine > key));
-          const uint64_t up = __shfl_up_sync(0xffffffffu, mine, 1);
-          if (lane == at) mine = key;
-          else if (lane > at) mine = up;
-        }
-      }
-    }
-  }
-  sync();  // everybody has read what was picked
-  if constexpr (kRowWarps > 1) {
-    if (lane < k) space.keys[warp * k + lane] = mine;
-    sync();
-    k_largest(space.keys, kRowWarps * k, space.best, k, t, 32 * kRowWarps, sync);
-  } else {
-    if (lane < k) space.best[lane] = mine;
-    sync();
-  }
 }
 
-// kRowWarps = kWarps: a row to each cluster of 1, 2, 4 or 8 blocks, each block with a run
-// of the row's chunks; the blocks' results are joined in the first block's
-// shared memory, in order.  kRowWarps = 1: a row to each warp, eight to a block.
+// kRowWarps > 1: a row to each cluster of 1, 2, 4 or 8 blocks of so many warps, each block
+// with a run of the row's chunks; the blocks' results are joined in the first
+// block's shared memory, in order.  kRowWarps = 1: a row to each warp, four to a block.
 //
 // One read of the row: a warp has kLoads chunks in flight, takes their maximum, and
 // adds up the sums on its scale.
+template <int kRowWarps>
+constexpr int kBlockWarps = kRowWarps == 1 ? 4 : kRowWarps;
+
 template <class T, int kRowWarps, bool kEntropy, bool kTop>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(32 * kBlockWarps<kRowWarps>)
     token_logprobs_kernel(const T* __restrict__ x, const ForwardArgs a, int64_t rows, int max_chunks) {
   pdl_entry();
   constexpr int kPer = Vec<T>::kPer, kPairs = kPer / 2;
-  constexpr int kRows = kWarps / kRowWarps;
-  extern __shared__ float chunk_maxima[];  // [kRows][max_chunks]
+  constexpr int kWarps = kBlockWarps<kRowWarps>, kRows = kWarps / kRowWarps;
+  extern __shared__ __align__(16) uint64_t top_scratch[];  // [kRows]: the runs' chunks, the chunks' maxima
   __shared__ Stats warp_stats[kWarps];
   __shared__ Stats part_stats[kRowWarps == 1 ? 1 : kMaxCluster];
-  __shared__ uint64_t part_best[kTop && kRowWarps > 1 ? kMaxCluster * MCKE_TOP_MAX : 1];
-  __shared__ TopSpace<kRowWarps> top_space[kTop ? kRows : 1];
+  __shared__ __align__(16) uint64_t part_best[kTop && kRowWarps > 1 ? kMaxCluster * MCKE_TOP_MAX : 1];
+  __shared__ TopSpace<kTop ? kRowWarps : 1> top_space[kTop ? kRows : 1];
   const int lane = threadIdx.x & 31, warp = kRowWarps == 1 ? 0 : threadIdx.x >> 5;
   const int slot = kRowWarps == 1 ? threadIdx.x >> 5 : 0;
   const uint32_t blocks = kRowWarps == 1 ? 1 : cluster_blocks(), block = kRowWarps == 1 ? 0 : cluster_block();
@@ -359,7 +423,9 @@ __global__ void __launch_bounds__(kThreads)
     if constexpr (kRowWarps == 1) __syncwarp();
     else __syncthreads();
   };
-  float* const chunk_max = chunk_maxima + slot * max_chunks;
+  const TopScratch scratch(max_chunks, 32 * kRowWarps);
+  uint64_t* const run_keys = top_scratch + slot * scratch.words;
+  float* const chunk_max = reinterpret_cast<float*>(run_keys + scratch.run_keys);
   const T* xr = x + row * a.stride;
   const int shift = vec_shift(xr);
   const int64_t vecs = (a.cols + shift + kPer - 1) / kPer;
@@ -438,10 +504,11 @@ __global__ void __launch_bounds__(kThreads)
   }
   sync();
   if constexpr (kTop)
-    top_of_part<T, kRowWarps>(xr, a.cols, chunk0 * 32, shift, chunk_max, chunks, a.top_k, top_space[slot], sync);
+    top_of_part<T, kRowWarps>(xr, a.cols, chunk0 * 32, shift, chunk_max, run_keys, chunks, a.top_k, top_space[slot],
+                              sync);
   const uint64_t* best = top_space[slot].best;
   if constexpr (kRowWarps > 1) {
-    // the warps' statistics, a lane to each: the same bits in every lane
+    // eight statistics, a lane to each: the same bits in every lane
     auto join_lanes = [&](Stats s8) {
 #pragma unroll
       for (int o = 4; o > 0; o >>= 1)
@@ -449,8 +516,9 @@ __global__ void __launch_bounds__(kThreads)
                             __shfl_xor_sync(0xffffffffu, s8.w, o)});
       return s8;
     };
-    static_assert(kWarps == 8 && kMaxCluster == 8, "eight lanes");
-    if (warp == 0) st = join_lanes(warp_stats[lane & 7]);
+    static_assert(kWarps <= 8 && kMaxCluster <= 8, "eight lanes");
+    const Stats nothing{-INFINITY, 0.0f, 0.0f};
+    if (warp == 0) st = join_lanes((lane & 7) < kWarps ? warp_stats[lane & 7] : nothing);
     if (blocks > 1) {
       cluster_barrier();  // every block of the cluster runs: its shared memory may be written
       if (threadIdx.x < 3) {
@@ -466,13 +534,14 @@ __global__ void __launch_bounds__(kThreads)
                      : "memory");
       cluster_barrier();
       if (block > 0) return;
+      // blocks * top_k is even
       if constexpr (kTop)
-        k_largest(part_best, static_cast<int>(blocks) * a.top_k, top_space[slot].best, a.top_k, threadIdx.x, kThreads,
-                  sync);
+        k_largest(part_best, static_cast<int>(blocks) * a.top_k, top_space[slot].best, a.top_k, threadIdx.x,
+                  32 * kWarps, sync);
     }
     if (warp > 0) return;
     if (blocks > 1)
-      st = join_lanes((lane & 7) < static_cast<int>(blocks) ? part_stats[lane & 7] : Stats{-INFINITY, 0.0f, 0.0f});
+      st = join_lanes((lane & 7) < static_cast<int>(blocks) ? part_stats[lane & 7] : nothing);
   }
   // a row of which nothing is left (with a NaN or +inf in it, m or s is not so)
   const bool none = st.m == -INFINITY;
@@ -587,42 +656,49 @@ __global__ void __launch_bounds__(kThreads, 6)
   }
 }
 
-// Blocks that share a row.  With few rows a row's time is that of one block's
-// share of it, so the row is spread until the blocks fill the device about once; a
-// block keeps at least a full round of loads.
-template <class T>
+// Blocks that share a row: 1, 2, 4 or 8, whichever takes the least time in rounds of
+// loads when the blocks run in waves over the device, with kTail rounds for what
+// a block does besides its loads.  With few rows that spreads a row over eight
+// blocks; with many it keeps the last wave from running half empty.
+template <class T, int kRowWarps, bool kTop>
 int row_blocks(int64_t rows, int64_t cols) {
-  const int64_t rounds = (cols + kThreads * kLoads * Vec<T>::kPer - 1) / (kThreads * kLoads * Vec<T>::kPer);
-  int n = 1;
-  while (n < kMaxCluster && 2 * n * rows <= 2 * 148 && n < rounds) n *= 2;
-  return n;
+  constexpr int64_t kRound = 32 * kRowWarps * kLoads * Vec<T>::kPer, kTail = kTop ? 4 : 2;
+  constexpr int64_t kResident = 148 * (48 / kRowWarps);  // at 40 registers a thread
+  const int64_t rounds = (cols + kRound - 1) / kRound;
+  int best = 1;
+  int64_t best_time = 0;
+  for (int n = 1; n <= kMaxCluster && n <= rounds; n *= 2) {
+    const int64_t time = ((rows * n + kResident - 1) / kResident) * ((rounds + n - 1) / n + kTail);
+    if (n == 1 || time < best_time) {
+      best = n;
+      best_time = time;
+    }
+  }
+  return best;
 }
-// A row to a warp where a block would have less than a round of loads for it and there
-// are rows enough for every SM's warps.
+// A row to a warp where a block would have few rounds of loads for it and there are
+// rows enough for every SM's warps.
 template <class T>
 bool warp_rows(int64_t rows, int64_t cols) {
-  return cols <= kWarpCols<T> && rows >= 148 * kWarps;
+  return cols <= kWarpCols<T> && rows >= 148 * 8;
 }
 
-template <class T, int kRowWarps>
+template <class T, int kRowWarps, bool kTop>
 void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
-  const int blocks = kRowWarps == 1 ? 1 : row_blocks<T>(rows, a.cols);
-  const bool top = a.top_k > 0;
+  const int blocks = kRowWarps == 1 ? 1 : row_blocks<T, kRowWarps, kTop>(rows, a.cols);
   // the chunk maxima of the largest part, whatever the row's shift
   const int64_t chunks = ((a.cols + Vec<T>::kPer - 1) / Vec<T>::kPer + 1 + 31) / 32;
-  const int max_chunks = top ? static_cast<int>((chunks + blocks - 1) / blocks + 1) : 0;
-  const std::size_t smem = static_cast<std::size_t>(max_chunks) * (kWarps / kRowWarps) * sizeof(float);
-  auto kernel = a.entropy ? (top ? token_logprobs_kernel<T, kRowWarps, true, true>
-                                 : token_logprobs_kernel<T, kRowWarps, true, false>)
-                          : (top ? token_logprobs_kernel<T, kRowWarps, false, true>
-                                 : token_logprobs_kernel<T, kRowWarps, false, false>);
+  const int max_chunks = kTop ? static_cast<int>((chunks + blocks - 1) / blocks + 1) : 0;
+  constexpr int kRows = kBlockWarps<kRowWarps> / kRowWarps;
+  const std::size_t smem = kTop ? static_cast<std::size_t>(TopScratch(max_chunks, 32 * kRowWarps).words) * kRows * 8 : 0;
+  auto kernel = a.entropy ? token_logprobs_kernel<T, kRowWarps, true, kTop> : token_logprobs_kernel<T, kRowWarps, false, kTop>;
   if (smem > 32 * 1024)
     cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
                          static_cast<int>(smem));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
-  cfg.gridDim = dim3(static_cast<unsigned>(kRowWarps == 1 ? (rows + kWarps - 1) / kWarps : rows * blocks));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>((rows + kRows - 1) / kRows * blocks));
+  cfg.blockDim = dim3(32 * kBlockWarps<kRowWarps>);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
@@ -639,10 +715,14 @@ void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t
   cudaLaunchKernelEx(&cfg, kernel, x, a, rows, max_chunks);  // errors are left for check_launch()
 }
 
+// With alternatives a row's end is long, and blocks of four warps leave more of them on
+// an SM to cover it (8192 x 32768 bf16 with five: 115 us against 138 with eight);
+// without, blocks of eight are the faster (89 us against 94).
 template <class T>
 void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
-  if (warp_rows<T>(rows, a.cols)) launch_forward<T, 1>(x, a, rows, s);
-  else launch_forward<T, kWarps>(x, a, rows, s);
+  const bool narrow = warp_rows<T>(rows, a.cols);
+  if (a.top_k > 0) narrow ? launch_forward<T, 1, true>(x, a, rows, s) : launch_forward<T, 4, true>(x, a, rows, s);
+  else narrow ? launch_forward<T, 1, false>(x, a, rows, s) : launch_forward<T, 8, false>(x, a, rows, s);
 }
 
 template <class T>
