@@ -5,17 +5,18 @@
 //
 // The list's table (pointers, lengths, types) travels in the launch's
 // parameters, so a call copies nothing to the device and a captured CUDA graph
-// holds all it needs.  Every tensor is cut into chunks of 1024 16-byte vectors
+// holds all it needs.  Every tensor is cut into chunks of 2048 16-byte vectors
 // (counted from the 16-byte boundary at or below its first element, so a tensor
-// may start anywhere), the chunks of all tensors are numbered through, and
-// each block takes one contiguous run of them: short tensors cost no launch and
-// no block of their own.
+// may start anywhere), the chunks of all tensors are numbered through, and the
+// blocks take them in turn: short tensors cost no launch and no block of their own,
+// and the blocks move through memory side by side.
 //
 // Squares are added in double: the sum neither loses small gradients next to
 // large ones nor leaves float's range where the norm itself does not.  The
-// blocks' sums go to the workspace and are folded in block order by every block
-// of the scaling kernel (or by the one block that only writes the norm).  The
-// grid follows from the extents alone, so the norm has the same bits on any GPU.
+// blocks' sums go to the workspace and are folded in block order, of a short list by
+// every block of the scaling kernel (one launch less), of a long one by a kernel
+// of one block.  The grid follows from the tensors alone, so the norm has the same
+// bits on any GPU.
 #include <algorithm>
 #include <new>
 #include <vector>
@@ -27,9 +28,15 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kChunkVecs = 1024;  // 16 KB
+constexpr int kChunkVecs = 2048;  // 32 KB
 constexpr int kUnroll = kChunkVecs / kThreads;
-constexpr int64_t kMaxBlocks = 8 * 148;
+// Blocks of the two passes at most.  The squares: what is resident at once, three to
+// an SM with two chunks each in flight (1.04 GB of bf16: 173 us, 191 us with five blocks of
+// 16 KB chunks, 227 us with six, which are more than fit).  Scaling: many short blocks,
+// so that none of a few long ones is the last (the same list: 306 us, 333 us with
+// six to an SM that stay).
+constexpr int64_t kMaxBlocks = 3 * 148;
+constexpr int64_t kClipBlocks = 64 * 148;
 constexpr float kNormEps = 1e-6f;
 
 struct Entry {
@@ -58,9 +65,11 @@ struct NormSource {
   float max_norm;
 };
 
-// The tensor that holds chunk c, by bisection.
+// The tensor that holds chunk c: tensor i if it is still that one, else by bisection.
 template <int kCap>
-__device__ __forceinline__ int find_entry(const Table<kCap>& t, uint32_t c) {
+__device__ __forceinline__ int find_entry(const Table<kCap>& t, uint32_t c, int i) {
+  const uint32_t end = i + 1 < t.count ? t.e[i + 1].first_chunk : t.chunks;
+  if (c >= t.e[i].first_chunk && c < end) return i;
   int lo = 0, hi = t.count - 1;
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -70,9 +79,8 @@ __device__ __forceinline__ int find_entry(const Table<kCap>& t, uint32_t c) {
   return lo;
 }
 
-// The 16-byte vector v of a tensor, counted from the boundary at or below its
-// first element: elements [first, first + kPer) of it, of which those in
-// [0, numel) exist.
+// 16-byte vectors of a tensor are counted from the boundary at or below its first
+// element, which is element -shift of that count.
 template <class T>
 struct Vec {
   static constexpr int kPer = 16 / sizeof(T);
@@ -81,20 +89,6 @@ struct Vec {
   }
 };
 
-__device__ __forceinline__ void unpack(uint4 q, float (&v)[4], const float*) {
-  v[0] = __uint_as_float(q.x);
-  v[1] = __uint_as_float(q.y);
-  v[2] = __uint_as_float(q.z);
-  v[3] = __uint_as_float(q.w);
-}
-__device__ __forceinline__ void unpack(uint4 q, float (&v)[8], const uint16_t*) {
-  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[2 * j] = bf16_lo(w[j]);
-    v[2 * j + 1] = bf16_hi(w[j]);
-  }
-}
 // Plain loads: in place, another element of the tensor may be written by this grid.
 __device__ __forceinline__ uint4 ld_u4(const void* p) {
   uint4 v;
@@ -104,52 +98,114 @@ __device__ __forceinline__ uint4 ld_u4(const void* p) {
                : "memory");
   return v;
 }
-
-// Values of vector `first / kPer` (zeros for elements that do not exist).
+// The vector that starts at element `first`; zeros where the tensor has no element.
 template <class T>
-__device__ __forceinline__ void load_vec(const T* data, int64_t first, int64_t numel, float (&v)[Vec<T>::kPer]) {
+__device__ __forceinline__ uint4 ld_part(const T* data, int64_t first, int64_t numel) {
+  constexpr int kPer = Vec<T>::kPer, kPerWord = kPer / 4;
+  if (first >= 0 && first + kPer <= numel) return ld_u4(data + first);
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    if (first + j < 0 || first + j >= numel) continue;
+    if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(data[first + j]);
+    else w[j / kPerWord] |= static_cast<uint32_t>(data[first + j]) << (16 * (j % kPerWord));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// This thread's kUnroll vectors of a chunk.
+template <class T>
+__device__ __forceinline__ void ld_chunk(const Entry& e, uint32_t c, uint4 (&q)[kUnroll]) {
   constexpr int kPer = Vec<T>::kPer;
-  if (first >= 0 && first + kPer <= numel) {
-    unpack(ld_u4(data + first), v, static_cast<const T*>(nullptr));
+  const T* data = reinterpret_cast<const T*>(e.data);
+  const int64_t first = (static_cast<int64_t>(c - e.first_chunk) * kChunkVecs + threadIdx.x) * kPer - Vec<T>::shift(e.data);
+  if (first >= 0 && first + ((kUnroll - 1) * kThreads + 1) * kPer <= e.numel) {
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) q[u] = ld_u4(data + first + u * kThreads * kPer);
   } else {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] = (first + j >= 0 && first + j < numel) ? ld_val(data + first + j) : 0.0f;
+    for (int u = 0; u < kUnroll; ++u) q[u] = ld_part(data, first + u * kThreads * kPer, e.numel);
   }
 }
 
-template <class T>
-__device__ __forceinline__ double chunk_squares(const Entry& e, uint32_t c) {
-  constexpr int kPer = Vec<T>::kPer;
-  const T* data = reinterpret_cast<const T*>(e.data);
-  const int64_t v0 = static_cast<int64_t>(c - e.first_chunk) * kChunkVecs + threadIdx.x;
-  const int shift = Vec<T>::shift(e.data);
-  double s = 0.0;
+// x 2^-896 as a double, from the bits of |x| moved to a double's places: exact for every
+// finite float, and without the conversion unit, which the bf16 stream would keep 63%
+// busy at three quarters of the copy rate.  An infinity or a NaN becomes a
+// finite value of 2^-768 and up.
+__device__ __forceinline__ double scaled_abs(uint32_t bits) {
+  return __hiloint2double(static_cast<int>((bits & 0x7fffffffu) >> 3), static_cast<int>(bits << 29));
+}
+constexpr double kUnscale = 0x1p896;
+__device__ __forceinline__ double add_square(uint32_t bits, double s) {
+  const double x = scaled_abs(bits) * kUnscale;
+  return fma(x, x, s);
+}
+__device__ __forceinline__ double add_squares(const uint4 (&q)[kUnroll], bool bf16, double s) {
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    float v[kPer];
-    load_vec(data, (v0 + u * kThreads) * kPer - shift, e.numel, v);
+    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) s = fma(static_cast<double>(v[j]), static_cast<double>(v[j]), s);
+    for (int j = 0; j < 4; ++j) {
+      if (bf16) s = add_square(w[j] << 16, s);
+      s = add_square(bf16 ? w[j] & 0xffff0000u : w[j], s);
+    }
   }
   return s;
 }
+__device__ __forceinline__ bool any_nan(const uint4 (&q)[kUnroll], bool bf16) {
+  bool nan = false;
+#pragma unroll
+  for (int u = 0; u < kUnroll; ++u) {
+    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float hi = __uint_as_float(bf16 ? w[j] & 0xffff0000u : w[j]), lo = __uint_as_float(bf16 ? w[j] << 16 : 0u);
+      nan = nan || hi != hi || lo != lo;
+    }
+  }
+  return nan;
+}
 
+// The squares of a block's chunks, the next chunk's loads in flight while one is added
+// up.  A sum of 2^256 and more may have had a NaN or an infinity for a finite value:
+// the norm is then infinite in float, unless the block, looking again, finds a NaN.
 template <int kCap>
 __global__ void __launch_bounds__(kThreads)
     grad_squares_kernel(const __grid_constant__ Table<kCap> t, double* __restrict__ sums) {
   pdl_entry();
   __shared__ double red[kWarps];
-  const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / gridDim.x);
-  const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * (blockIdx.x + 1) / gridDim.x);
+  int i = 0;
+  auto load = [&](uint32_t c, uint4 (&q)[kUnroll]) {
+    i = find_entry(t, c, i);
+    const Entry& e = t.e[i];
+    if (e.bf16) ld_chunk<uint16_t>(e, c, q);
+    else ld_chunk<float>(e, c, q);
+    return e.bf16 != 0;
+  };
   double s = 0.0;
-  if (c0 < c1) {
-    int i = find_entry(t, c0);
-    for (uint32_t c = c0; c < c1; ++c) {
-      while (i + 1 < t.count && t.e[i + 1].first_chunk <= c) ++i;
-      s += t.e[i].bf16 ? chunk_squares<uint16_t>(t.e[i], c) : chunk_squares<float>(t.e[i], c);
+  if (blockIdx.x < t.chunks) {
+    uint4 q[kUnroll], next[kUnroll];
+    bool bf16 = load(blockIdx.x, q);
+    for (uint32_t c = blockIdx.x;;) {
+      c += gridDim.x;
+      bool next_bf16 = false;
+      if (c < t.chunks) next_bf16 = load(c, next);
+      s = bf16 ? add_squares(q, true, s) : add_squares(q, false, s);
+      if (c >= t.chunks) break;
+      bf16 = next_bf16;
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) q[u] = next[u];
     }
   }
   s = block_all_sum<kWarps>(s, red);
+  if (s >= 0x1p256) {
+    bool nan = false;
+    for (uint32_t c = blockIdx.x; c < t.chunks; c += gridDim.x) {
+      uint4 q[kUnroll];
+      const bool bf16 = load(c, q);
+      nan = nan || any_nan(q, bf16);
+    }
+    s = __syncthreads_or(nan) ? static_cast<double>(NAN) : static_cast<double>(INFINITY);
+  }
   if (threadIdx.x == 0) sums[blockIdx.x] = s;
 }
 
@@ -194,19 +250,26 @@ __device__ __forceinline__ void store_vec(uint16_t* out, int64_t first, int64_t 
 template <class T, class U>
 __device__ __forceinline__ void chunk_scale(const Entry& e, uint32_t c, float coef) {
   constexpr int kPer = Vec<T>::kPer;
-  const T* data = reinterpret_cast<const T*>(e.data);
   U* out = reinterpret_cast<U*>(e.out);
-  const int64_t v0 = static_cast<int64_t>(c - e.first_chunk) * kChunkVecs + threadIdx.x;
   const int shift = Vec<T>::shift(e.data);
+  const int64_t first = (static_cast<int64_t>(c - e.first_chunk) * kChunkVecs + threadIdx.x) * kPer - shift;
   const bool whole = ((reinterpret_cast<uintptr_t>(e.out) - shift * sizeof(U)) & 15) == 0;
+  uint4 q[kUnroll];
+  ld_chunk<T>(e, c, q);
 #pragma unroll
   for (int u = 0; u < kUnroll; ++u) {
-    const int64_t first = (v0 + u * kThreads) * kPer - shift;
+    const uint32_t w[4] = {q[u].x, q[u].y, q[u].z, q[u].w};
     float v[kPer];
-    load_vec(data, first, e.numel, v);
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) v[j] *= coef;
-    store_vec(out, first, e.numel, v, kPer, whole);
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (sizeof(T) == 4) {
+        v[j] = coef * __uint_as_float(w[j]);
+      } else {
+        v[2 * j] = coef * bf16_lo(w[j]);
+        v[2 * j + 1] = coef * bf16_hi(w[j]);
+      }
+    }
+    store_vec(out, first + u * kThreads * kPer, e.numel, v, kPer, whole);
   }
 }
 
@@ -220,12 +283,11 @@ __global__ void __launch_bounds__(kThreads)
   // a NaN norm stays NaN (fminf would return 1)
   const float ratio = src.max_norm / (n + kNormEps);
   const float coef = ratio > 1.0f ? 1.0f : ratio;
-  const uint32_t c0 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * blockIdx.x / gridDim.x);
-  const uint32_t c1 = static_cast<uint32_t>(static_cast<uint64_t>(t.chunks) * (blockIdx.x + 1) / gridDim.x);
-  if (c0 >= c1) return;
-  int i = find_entry(t, c0);
-  for (uint32_t c = c0; c < c1; ++c) {
-    while (i + 1 < t.count && t.e[i + 1].first_chunk <= c) ++i;
+  // the last chunks first: the norm's pass has left them in L2
+  int i = 0;
+  for (uint32_t n = blockIdx.x; n < t.chunks; n += gridDim.x) {
+    const uint32_t c = t.chunks - 1 - n;
+    i = find_entry(t, c, i);
     const Entry& e = t.e[i];
     if (coef == 1.0f && e.out == e.data) continue;  // 1 x is x: nothing to write
     if (!e.bf16) chunk_scale<float, float>(e, c, coef);
@@ -244,7 +306,7 @@ int64_t chunks_of(const mcke_grad& g) {
   return (vecs + kChunkVecs - 1) / kChunkVecs;
 }
 
-int64_t blocks_of(int64_t chunks) { return chunks < 1 ? 1 : chunks < kMaxBlocks ? chunks : kMaxBlocks; }
+int64_t blocks_of(int64_t chunks, int64_t most) { return chunks < 1 ? 1 : chunks < most ? chunks : most; }
 
 // One launch's share of the list: grads [begin, end), tensors of no element left out.
 template <int kCap>
@@ -265,7 +327,7 @@ template <int kCap>
 int64_t launch_squares(const mcke_grad* g, int begin, int end, double* sums, cudaStream_t s) {
   Table<kCap> t;
   fill(t, g, begin, end);
-  const int64_t blocks = blocks_of(t.chunks);
+  const int64_t blocks = blocks_of(t.chunks, kMaxBlocks);
   launch_async(grad_squares_kernel<kCap>, static_cast<unsigned>(blocks), kThreads, 0, s, t, sums);
   return blocks;
 }
@@ -273,7 +335,7 @@ template <int kCap>
 void launch_clip(const mcke_grad* g, int begin, int end, const NormSource& src, cudaStream_t s) {
   Table<kCap> t;
   fill(t, g, begin, end);
-  launch_async(grad_clip_kernel<kCap>, static_cast<unsigned>(blocks_of(t.chunks)), kThreads, 0, s, t, src);
+  launch_async(grad_clip_kernel<kCap>, static_cast<unsigned>(blocks_of(t.chunks, kClipBlocks)), kThreads, 0, s, t, src);
 }
 
 // Sums of squares of the whole list; returns how many sums were written.
@@ -423,6 +485,12 @@ extern "C" int mcke_sm100_clip_grad_norm(const mcke_grad* grads, int count, floa
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   double* sums = static_cast<double*>(workspace);
   const int n = all_squares(grads, count, sums, s);
-  all_clip(grads, count, NormSource{sums, n, nullptr, norm, max_norm}, s);
+  if (n < kMaxBlocks) {
+    all_clip(grads, count, NormSource{sums, n, nullptr, norm, max_norm}, s);
+  } else {
+    // more blocks than fit at once: folded once for all of them
+    launch_async(grad_norm_fold_kernel, 1, kThreads, 0, s, static_cast<const double*>(sums), n, norm);
+    all_clip(grads, count, NormSource{nullptr, 0, norm, nullptr, max_norm}, s);
+  }
   return check_launch(who);
 }
