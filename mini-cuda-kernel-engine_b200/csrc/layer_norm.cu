@@ -729,6 +729,34 @@ struct BackwardArgs {
   int rows, cols;
 };
 
+// Adds the groups' column sums, kN pairs of dw and db to a thread, to the first group's, in
+// group order.  cell: (kGroups - 1) * 2 kN * kTpg pairs of shared memory that the whole
+// block is done with.  False for the other groups' threads.
+template <int kGroups, int kTpg, int kN>
+__device__ __forceinline__ bool join_groups(F2* cell, int group, F2* dw, F2* db) {
+  if constexpr (kGroups > 1) {
+    cell += threadIdx.x % kTpg;  // [group - 1][dw, db][pair][thread]
+    __syncthreads();
+    if (group > 0) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        cell[((group - 1) * 2 * kN + i) * kTpg] = dw[i];
+        cell[((group - 1) * 2 * kN + kN + i) * kTpg] = db[i];
+      }
+    }
+    __syncthreads();
+    if (group > 0) return false;
+    for (int g = 0; g < kGroups - 1; ++g) {
+#pragma unroll
+      for (int i = 0; i < kN; ++i) {
+        dw[i] = add2(dw[i], cell[(g * 2 * kN + i) * kTpg]);
+        db[i] = add2(db[i], cell[(g * 2 * kN + kN + i) * kTpg]);
+      }
+    }
+  }
+  return true;
+}
+
 // dx, and the column sums of each slab (the rows of one cluster), in one read of dy
 // and x: a thread adds up its 16 columns in registers over all its rows, the
 // block's groups are added in shared memory at the end.  Each turn of the loop
@@ -876,37 +904,8 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
   copies_wait<0>();
   if constexpr (kCluster > 1) cluster_barrier();  // no block leaves while another's post may be on its way to it
   if (!a.part) return;
-  // the groups' column sums, added in group order
-  if constexpr (kGroups > 1) {
-    __syncthreads();
-    F2* const cell = reinterpret_cast<F2*>(ring);  // [group - 1][dw, db][unit][pair][thread]
-    static_assert(2 * kUnits * kPairs * 8 <= static_cast<int>(S::kSmem / S::kThreads), "the ring holds the groups' sums");
-    auto at = [&](int g, int which, int i, int j) {
-      return cell + ((((g - 1) * 2 + which) * kUnits + i) * kPairs + j) * S::kTpg + threadIdx.x % S::kTpg;
-    };
-    if (group > 0) {
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          *at(group, 0, i, j) = dw[i][j];
-          *at(group, 1, i, j) = db[i][j];
-        }
-      }
-    }
-    __syncthreads();
-    if (group > 0) return;
-    for (int g = 1; g < kGroups; ++g) {
-#pragma unroll
-      for (int i = 0; i < kUnits; ++i) {
-#pragma unroll
-        for (int j = 0; j < kPairs; ++j) {
-          dw[i][j] = add2(dw[i][j], *at(g, 0, i, j));
-          db[i][j] = add2(db[i][j], *at(g, 1, i, j));
-        }
-      }
-    }
-  }
+  static_assert(2 * kUnits * kPairs * 8 <= static_cast<int>(S::kSmem / S::kThreads), "the ring holds the groups' sums");
+  if (!join_groups<kGroups, S::kTpg, kUnits * kPairs>(reinterpret_cast<F2*>(ring), group, &dw[0][0], &db[0][0])) return;
   float* const out = a.part + static_cast<int64_t>(cluster) * 2 * a.cols + t * kPer;
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
@@ -916,6 +915,120 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
       const float2 a0 = split(dw[i][j]), a1 = split(dw[i][j + 1]), b0 = split(db[i][j]), b1 = split(db[i][j + 1]);
       *reinterpret_cast<float4*>(out + i * kTpr * kPer + 2 * j) = make_float4(a0.x, a0.y, a1.x, a1.y);
       *reinterpret_cast<float4*>(out + a.cols + i * kTpr * kPer + 2 * j) = make_float4(b0.x, b0.y, b1.x, b1.y);
+    }
+  }
+}
+
+// The same for rows that are not whole 16-byte units: consecutive threads have consecutive
+// elements, 16 of them in pairs (of columns c and c + kTpg).  Elements of the row after
+// next come into registers (two bytes are less than an asynchronous copy moves) and go
+// to the ring, of the last row, this one and the next, a turn later.
+template <class T, int kW, int kGroups>
+__global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elements_kernel(const BackwardArgs a) {
+  pdl_entry();
+  constexpr int kPairs = 8, kTpg = 32 * kW, kThr = kTpg * kGroups, kStages = 3;
+  extern __shared__ __align__(16) uint4 ring[];  // T [stage][dy, x][element][thread]
+  __shared__ PostedSums<2, kW, 1> posted[kGroups];
+  const int group = threadIdx.x / kTpg, t = threadIdx.x % kTpg;
+  auto col = [&](int e) { return e * kTpg + t; };
+  const int step = gridDim.x * kGroups;
+  int row = blockIdx.x + gridDim.x * group;
+  if (t == 0) init_sums(posted[group]);
+  __syncthreads();
+  T* const cells = reinterpret_cast<T*>(ring) + threadIdx.x;
+  auto cell = [&](int stage, int operand, int e) { return cells + ((stage * 2 + operand) * 2 * kPairs + e) * kThr; };
+  T dyr[2 * kPairs], xr[2 * kPairs];
+  auto load = [&](int64_t r) {
+    if (r >= a.rows) return;
+    const T* dy = static_cast<const T*>(a.dy) + r * a.dy_stride;
+    const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
+#pragma unroll
+    for (int e = 0; e < 2 * kPairs; ++e) {
+      dyr[e] = col(e) < a.cols ? __ldg(dy + col(e)) : T(0);
+      xr[e] = col(e) < a.cols ? __ldg(x + col(e)) : T(0);
+    }
+  };
+  auto store = [&](int stage) {
+#pragma unroll
+    for (int e = 0; e < 2 * kPairs; ++e) {
+      *cell(stage, 0, e) = dyr[e];
+      *cell(stage, 1, e) = xr[e];
+    }
+  };
+  load(row);
+  F2 w[kPairs], dw[kPairs], db[kPairs];
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const int lo = col(2 * i), hi = col(2 * i + 1);
+    w[i] = f2(a.weight && lo < a.cols ? __ldg(a.weight + lo) : 1.0f, a.weight && hi < a.cols ? __ldg(a.weight + hi) : 1.0f);
+    dw[i] = db[i] = f2(0.0f);
+  }
+  store(0);
+  load(row + step);
+  const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
+  auto mean_of = [&](int r) { return r < a.rows ? __ldg(a.mean + r) : 0.0f; };
+  auto rstd_of = [&](int r) { return r < a.rows ? __ldg(a.rstd + r) : 0.0f; };
+  float mu = mean_of(row), r = rstd_of(row), last_mu = 0.0f, last_r = 0.0f;
+  int stage = 0, last_stage = 0;
+  for (int turn = 0; row < a.rows + step; ++turn, row += step) {
+    const float next_mu = mean_of(row + step), next_r = rstd_of(row + step);
+    if (row < a.rows) {
+      const F2 minus_mu = f2(-mu), rr = f2(r);
+      F2 s1 = f2(0.0f), s2 = f2(0.0f);
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        // columns past the row have dy = 0 and add nothing
+        const F2 d = f2(ld_val(cell(stage, 0, 2 * i)), ld_val(cell(stage, 0, 2 * i + 1)));
+        const F2 v = f2(ld_val(cell(stage, 1, 2 * i)), ld_val(cell(stage, 1, 2 * i + 1)));
+        const F2 p = mul2(d, add2(v, minus_mu));
+        db[i] = add2(db[i], d);
+        dw[i] = fma2(p, rr, dw[i]);
+        s1 = fma2(d, w[i], s1);
+        s2 = fma2(p, w[i], s2);
+      }
+      const float sums[2] = {sum2(s1), sum2(s2)};
+      post_sums(sums, posted[group], turn % kPlaces);
+    }
+    const int next_stage = stage + 1 == kStages ? 0 : stage + 1;
+    if (turn > 0) {
+      float c[2];
+      collect_sums(c, posted[group], (turn - 1) % kPlaces, static_cast<uint32_t>((turn - 1) / kPlaces) & 1u);
+      const F2 minus_mu = f2(-last_mu), rr = f2(last_r);
+      const F2 k1 = f2(-last_r * div_by(c[0], n, inv_n));
+      const F2 k2 = f2(-last_r * last_r * (last_r * div_by(c[1], n, inv_n)));
+      T* dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row - step) * a.dx_stride;
+#pragma unroll
+      for (int i = 0; i < kPairs; ++i) {
+        if (col(2 * i) >= a.cols) break;
+        const F2 d = f2(ld_val(cell(last_stage, 0, 2 * i)), ld_val(cell(last_stage, 0, 2 * i + 1)));
+        const F2 v = f2(ld_val(cell(last_stage, 1, 2 * i)), ld_val(cell(last_stage, 1, 2 * i + 1)));
+        const float2 g = split(fma2(add2(v, minus_mu), k2, fma2(mul2(d, w[i]), rr, k1)));
+        st_val(dx + col(2 * i), g.x);
+        if (col(2 * i + 1) < a.cols) st_val(dx + col(2 * i + 1), g.y);
+      }
+    }
+    store(next_stage);
+    load(static_cast<int64_t>(row) + 2 * step);
+    last_mu = mu;
+    last_r = r;
+    mu = next_mu;
+    r = next_r;
+    last_stage = stage;
+    stage = next_stage;
+  }
+  if (!a.part) return;
+  if (!join_groups<kGroups, kTpg, kPairs>(reinterpret_cast<F2*>(ring), group, dw, db)) return;
+  float* const out = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) {
+    const float2 x = split(dw[i]), b = split(db[i]);
+    if (col(2 * i) < a.cols) {
+      out[col(2 * i)] = x.x;
+      out[a.cols + col(2 * i)] = b.x;
+    }
+    if (col(2 * i + 1) < a.cols) {
+      out[col(2 * i + 1)] = x.y;
+      out[a.cols + col(2 * i + 1)] = b.y;
     }
   }
 }
@@ -1104,7 +1217,7 @@ int64_t launch_stream(void (*kernel)(const A), const A& a, int64_t items, int th
 
 // Calls f(warps, blocks) with the smallest group, of 1 .. 16 warps in each of 1, 2 or 4
 // blocks, whose threads hold a row of `cols` <= kStreamCols at 16 elements each.
-constexpr int64_t kStreamCols = 4 * 8192;
+constexpr int64_t kStreamCols = 4 * 8192, kElementCols = 8192;
 template <class F>
 void with_group(int64_t cols, F&& f) {
   using std::integral_constant;
@@ -1221,6 +1334,18 @@ void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* d
   int64_t slabs = 0;
   if (a.rows > 0 && whole && a.cols <= kStreamCols) {
     slabs = launch_backward_stream<T>(a, s);
+  } else if (a.rows > 0 && a.cols <= kElementCols) {
+    with_group(a.cols, [&](auto warps, auto blocks) {
+      constexpr int kW = decltype(warps)::value;
+      if constexpr (decltype(blocks)::value == 1) {
+        constexpr int kGroups = kW == 1 ? 15 : 16 / kW;
+        // the ring, or at the end the groups' sums
+        constexpr std::size_t kRing = 3 * 2 * 16 * 32 * kW * kGroups * sizeof(T);
+        constexpr std::size_t kSums = static_cast<std::size_t>(kGroups - 1) * 32 * 32 * kW * sizeof(float);
+        slabs = launch_stream<1>(layer_norm_backward_elements_kernel<T, kW, kGroups>, a, a.rows, 32 * kW * kGroups,
+                                 kRing > kSums ? kRing : kSums, s);
+      }
+    });
   } else if (a.rows > 0) {
     launch_async(layer_norm_dx_kernel<T>, static_cast<unsigned>(a.rows), kThreads, 0, s, dy, a.dy_stride, x, a.x_stride,
                  a.weight, a.mean, a.rstd, static_cast<T*>(a.dx), a.dx_stride, static_cast<int64_t>(a.cols));
