@@ -390,7 +390,7 @@ int check_list(const char* who, const mcke_grad* g, int count, bool writes, cons
     chunks += chunks_of(g[i]);
     if (chunks > 2147483647LL) return fail(MCKE_INVALID_ARGUMENT, "%s: the list holds too many elements", who);
   }
-  if (!writes && !norm_out) return MCKE_OK;
+  if (!aligned(norm, 4)) return fail(MCKE_INVALID_ARGUMENT, "%s: norm is not element-aligned", who);
   try {
     std::vector<Interval> v;
     v.reserve(2 * static_cast<size_t>(count) + 2);

@@ -9,8 +9,11 @@
 // Statistics and sums are float whatever the tensors' type; y and dx are rounded
 // once.  The variance is the mean of the squared deviations from the row's
 // mean, not a difference of two large sums.
-#include <initializer_list>
+#include <map>
+#include <mutex>
+#include <new>
 #include <type_traits>
+#include <utility>
 
 #include "row_ops.cuh"
 
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel
   using U = Unit<T>;
   constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
   using S = Stream<T, kUnits, kW, kGroups, kStages, 2>;
-  extern __shared__ __align__(16) uint4 ring[];
+  extern __shared__ __align__(128) uint4 ring[];
   __shared__ GroupSums<kW> red[kGroups];
   constexpr int kTpr = S::kTpg;
   const int group = threadIdx.x / S::kTpg, t = threadIdx.x % S::kTpg;
@@ -483,6 +486,7 @@ struct PostedSums {
   static constexpr int kPerLane = (kEntries + 7) / 8;
   float share[kPlaces][kN][8 * kPerLane];
   uint64_t arrived[kPlaces];
+  volatile int gave_up;  // a wait has run out: the later ones do not wait
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
@@ -497,6 +501,7 @@ __device__ __forceinline__ uint32_t in_block(uint32_t address, uint32_t block) {
 // By one thread, before any warp of the cluster posts.
 template <int kN, int kW, int kCluster>
 __device__ __forceinline__ void init_sums(PostedSums<kN, kW, kCluster>& p) {
+  p.gave_up = 0;
   for (int k = 0; k < kPlaces; ++k)
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&p.arrived[k])), "r"(kW) : "memory");
 }
@@ -546,24 +551,26 @@ __device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t phase) {
   return done != 0;
 }
 
-// Waits (2 s at most; a wait that runs out is recorded and passed, and the sums are
-// then incomplete) until every share of place k is there, and returns the sums: the
-// same bits in every thread.
-template <int kN, int kW, int kCluster>
-__device__ __forceinline__ void collect_sums(float (&v)[kN], const PostedSums<kN, kW, kCluster>& p, int k,
-                                             uint32_t phase) {
-  const uint32_t bar = shared_address(&p.arrived[k]);
-  if (!try_phase(bar, phase)) {
-    unsigned long long t0, t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-    while (!try_phase(bar, phase)) {
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t - t0 > kWaitNs) {
-        atomicCAS(&g_layer_norm_watchdog, 0u, 1u);
-        break;
-      }
+// Waits, 2 s at most: a wait that runs out is recorded and passed, as are all later ones
+// of the group, whose sums are then incomplete.
+__device__ __noinline__ void wait_phase(uint32_t bar, uint32_t phase, volatile int* gave_up) {
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  while (!*gave_up && !try_phase(bar, phase)) {
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t - t0 > kWaitNs) {
+      *gave_up = 1;
+      atomicCAS(&g_layer_norm_watchdog, 0u, 1u);
     }
   }
+}
+
+// Waits until every share of place k is there, and returns the sums: the
+// same bits in every thread.
+template <int kN, int kW, int kCluster>
+__device__ __forceinline__ void collect_sums(float (&v)[kN], PostedSums<kN, kW, kCluster>& p, int k, uint32_t phase) {
+  const uint32_t bar = shared_address(&p.arrived[k]);
+  if (!try_phase(bar, phase)) wait_phase(bar, phase, &p.gave_up);
   using P = PostedSums<kN, kW, kCluster>;
   const int lane = threadIdx.x & 31, at = (lane & 7) * P::kPerLane;
   const float* mine = p.share[k][(lane >> 3) % kN] + at;
@@ -588,7 +595,7 @@ __global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const Fo
   using U = Unit<T>;
   constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
   using S = Stream<T, kUnits, kW, 1, kStages, kRows>;
-  extern __shared__ __align__(16) uint4 ring[];
+  extern __shared__ __align__(128) uint4 ring[];
   __shared__ PostedSums<2 * kRows, kW, kCluster> posted;
   constexpr int kTpr = S::kTpg * kCluster;  // the row's threads of all blocks
   const int t = threadIdx.x + static_cast<int>(block_in_cluster()) * S::kTpg;
@@ -768,7 +775,7 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
   using U = Unit<T>;
   constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
   using S = Stream<T, kUnits, kW, kGroups, kStages, 2 * kRows>;
-  extern __shared__ __align__(16) uint4 ring[];
+  extern __shared__ __align__(128) uint4 ring[];
   __shared__ PostedSums<2 * kRows, kW, kCluster> posted[kGroups];
   constexpr int kTpr = S::kTpg * kCluster;
   const int group = threadIdx.x / S::kTpg;
@@ -927,7 +934,7 @@ template <class T, int kW, int kGroups>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elements_kernel(const BackwardArgs a) {
   pdl_entry();
   constexpr int kPairs = 8, kTpg = 32 * kW, kThr = kTpg * kGroups, kStages = 3;
-  extern __shared__ __align__(16) uint4 ring[];  // T [stage][dy, x][element][thread]
+  extern __shared__ __align__(128) uint4 ring[];  // T [stage][dy, x][element][thread]
   __shared__ PostedSums<2, kW, 1> posted[kGroups];
   const int group = threadIdx.x / kTpg, t = threadIdx.x % kTpg;
   auto col = [&](int e) { return e * kTpg + t; };
@@ -1185,9 +1192,7 @@ void with_count(int64_t n, F&& f) {
 // clusters as there are items, kStreamBlocks blocks at most.  Returns the clusters.
 template <int kCluster, class A>
 int64_t launch_stream(void (*kernel)(const A), const A& a, int64_t items, int threads, std::size_t smem, cudaStream_t s) {
-  // the attribute is a property of the kernel on the current device: set it every time
-  cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                       static_cast<int>(smem));
+  allow_shared_memory(reinterpret_cast<const void*>(kernel), smem);  // a launch that lacks it fails
   // 33 clusters of four fit a B200 (its 148 SMs come in groups that four does not
   // divide), 74 of two
   constexpr int64_t kMost = kCluster == 4 ? 32 : kStreamBlocks / kCluster;
@@ -1366,6 +1371,25 @@ void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* d
 }  // namespace mcke_sm100
 
 namespace mcke_sm100 {
+bool allow_shared_memory(const void* kernel, std::size_t bytes) {
+  static std::mutex mu;
+  static std::map<std::pair<const void*, int>, std::size_t> done;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return false;
+  std::lock_guard<std::mutex> lk(mu);
+  try {
+    std::size_t& most = done[{kernel, dev}];
+    if (bytes <= most) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) != cudaSuccess)
+      return false;
+    most = bytes;
+    return true;
+  } catch (const std::bad_alloc&) {  // no room to remember it
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes)) ==
+           cudaSuccess;
+  }
+}
+
 // Reads and clears the word that an expired wait of the backward pass sets.
 int read_layer_norm_watchdog(uint32_t* site) {
   uint32_t v = 0;
@@ -1393,12 +1417,13 @@ extern "C" int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const floa
   if (!(eps >= 0.0f) || std::isinf(eps)) return fail(MCKE_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", who);
   if (rows == 0 || cols == 0) return MCKE_OK;
   if (!x || !y) return fail(MCKE_INVALID_ARGUMENT, "%s: null pointer", who);
-  if (rows > 2147483647LL || cols > 2147483647LL)
-    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX", who);
+  if (rows > kMaxRows || cols > 2147483647LL)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX (rows: 65536 less)", who);
   MCKE_RETURN_IF(check_stride(who, "x", x_stride, rows, cols, false));
   MCKE_RETURN_IF(check_stride(who, "y", y_stride, rows, cols, true));
   const std::size_t e = dtype_bytes(dtype);
-  if (!aligned(x, e) || !aligned(y, e)) return fail(MCKE_INVALID_ARGUMENT, "%s: x or y is not element-aligned", who);
+  MCKE_RETURN_IF(check_aligned(
+      who, {{"x", x, e}, {"y", y, e}, {"weight", weight, 4}, {"bias", bias, 4}, {"mean", mean, 4}, {"rstd", rstd, 4}}));
   const RowSpan outs[] = {span_of("y", y, rows, cols, y_stride, e), span_of("mean", mean, rows * 4),
                           span_of("rstd", rstd, rows * 4)};
   const RowSpan ins[] = {span_of("x", x, rows, cols, x_stride, e), span_of("weight", weight, cols * 4),
@@ -1428,15 +1453,15 @@ extern "C" int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride,
   MCKE_RETURN_IF(check_dtype(who, dtype));
   if (rows < 0 || cols < 0) return fail(MCKE_INVALID_ARGUMENT, "%s: negative extent", who);
   if (cols == 0) return MCKE_OK;
-  if (rows > 2147483647LL || cols > 2147483647LL)
-    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX", who);
+  if (rows > kMaxRows || cols > 2147483647LL)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX (rows: 65536 less)", who);
   if (rows > 0 && (!dy || !x || !mean || !rstd || !dx)) return fail(MCKE_INVALID_ARGUMENT, "%s: null pointer", who);
   MCKE_RETURN_IF(check_stride(who, "dy", dy_stride, rows, cols, false));
   MCKE_RETURN_IF(check_stride(who, "x", x_stride, rows, cols, false));
   MCKE_RETURN_IF(check_stride(who, "dx", dx_stride, rows, cols, true));
   const std::size_t e = dtype_bytes(dtype);
-  if (!aligned(dy, e) || !aligned(x, e) || !aligned(dx, e))
-    return fail(MCKE_INVALID_ARGUMENT, "%s: dy, x or dx is not element-aligned", who);
+  MCKE_RETURN_IF(check_aligned(who, {{"dy", dy, e}, {"x", x, e}, {"dx", dx, e}, {"weight", weight, 4}, {"mean", mean, 4},
+                                     {"rstd", rstd, 4}, {"dweight", dweight, 4}, {"dbias", dbias, 4}}));
   const bool params = dweight || dbias;
   const size_t need = params ? mcke_sm100_layer_norm_backward_workspace_bytes(rows, cols) : 0;
   if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))

@@ -4,6 +4,7 @@
 #pragma once
 
 #include <cmath>
+#include <initializer_list>
 
 #include "mcke_common.cuh"
 
@@ -72,6 +73,25 @@ inline int check_stride(const char* who, const char* name, int64_t stride, int64
     return fail(MCKE_INVALID_ARGUMENT, "%s: %s spans more than 2^40 elements", who, name);
   return MCKE_OK;
 }
+
+// Rows of one launch: row numbers plus a step over all blocks stay below 2^31.
+constexpr int64_t kMaxRows = 2147483647LL - (1 << 16);
+
+// Vectors of 4- or 8-byte elements, null allowed.
+struct Aligned {
+  const char* name;
+  const void* p;
+  std::size_t bytes;
+};
+inline int check_aligned(const char* who, std::initializer_list<Aligned> list) {
+  for (const Aligned& v : list)
+    if (v.p && !aligned(v.p, v.bytes)) return fail(MCKE_INVALID_ARGUMENT, "%s: %s is not element-aligned", who, v.name);
+  return MCKE_OK;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device; one call
+// to the runtime per kernel and device.
+bool allow_shared_memory(const void* kernel, std::size_t bytes);
 
 // ---- device: elements ---------------------------------------------------------------
 

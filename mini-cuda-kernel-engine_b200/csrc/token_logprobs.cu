@@ -692,9 +692,7 @@ void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t
   constexpr int kRows = kBlockWarps<kRowWarps> / kRowWarps;
   const std::size_t smem = kTop ? static_cast<std::size_t>(TopScratch(max_chunks, 32 * kRowWarps).words) * kRows * 8 : 0;
   auto kernel = a.entropy ? token_logprobs_kernel<T, kRowWarps, true, kTop> : token_logprobs_kernel<T, kRowWarps, false, kTop>;
-  if (smem > 32 * 1024)
-    cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                         static_cast<int>(smem));
+  if (smem > 32 * 1024) allow_shared_memory(reinterpret_cast<const void*>(kernel), smem);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   cfg.gridDim = dim3(static_cast<unsigned>((rows + kRows - 1) / kRows * blocks));
@@ -762,8 +760,8 @@ extern "C" int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int
     return fail(MCKE_INVALID_ARGUMENT, "%s: top_k must be 0 .. %d", who, MCKE_TOP_MAX);
   if (rows == 0) return MCKE_OK;
   if (cols == 0) return fail(MCKE_INVALID_ARGUMENT, "%s: rows of no columns have no distribution", who);
-  if (rows > 2147483647LL || cols > 2147483647LL)
-    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX", who);
+  if (rows > kMaxRows || cols > 2147483647LL)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX (rows: 65536 less)", who);
   if (top_k > cols) return fail(MCKE_INVALID_ARGUMENT, "%s: top_k %d of %lld columns", who, top_k, static_cast<long long>(cols));
   if (top_k > 0 && cols > MCKE_TOP_COLS_MAX)
     return fail(MCKE_INVALID_ARGUMENT, "%s: top_k of more than %d columns", who, MCKE_TOP_COLS_MAX);
@@ -772,7 +770,9 @@ extern "C" int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int
   if (!logprobs && !lse && !entropy && top_k == 0) return MCKE_OK;
   MCKE_RETURN_IF(check_stride(who, "logits", stride, rows, cols, false));
   const std::size_t e = dtype_bytes(dtype);
-  if (!aligned(logits, e)) return fail(MCKE_INVALID_ARGUMENT, "%s: logits is not element-aligned", who);
+  MCKE_RETURN_IF(check_aligned(who, {{"logits", logits, e}, {"targets", targets, 8}, {"logprobs", logprobs, 4},
+                                     {"lse", lse, 4}, {"entropy", entropy, 4},
+                                     {"top_logprobs", top_logprobs, 4}, {"top_ids", top_ids, 8}}));
   const RowSpan outs[] = {span_of("logprobs", logprobs, rows * 4), span_of("lse", lse, rows * 4),
                           span_of("entropy", entropy, rows * 4),
                           span_of("top_logprobs", top_k > 0 ? top_logprobs : nullptr, rows * top_k * 4),
@@ -796,8 +796,8 @@ extern "C" int mcke_sm100_token_logprobs_backward(const void* logits, int64_t st
   MCKE_RETURN_IF(check_dtype(who, dtype));
   if (rows < 0 || cols < 0) return fail(MCKE_INVALID_ARGUMENT, "%s: negative extent", who);
   if (rows == 0 || cols == 0) return MCKE_OK;
-  if (rows > 2147483647LL || cols > 2147483647LL)
-    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX", who);
+  if (rows > kMaxRows || cols > 2147483647LL)
+    return fail(MCKE_INVALID_ARGUMENT, "%s: extent exceeds INT32_MAX (rows: 65536 less)", who);
   if (!logits || !lse || !dlogits || (grad_logprobs && !targets) || (grad_entropy && !entropy))
     return fail(MCKE_INVALID_ARGUMENT, "%s: null pointer", who);
   if (!grad_logprobs && !grad_entropy && !grad_lse)
@@ -805,8 +805,10 @@ extern "C" int mcke_sm100_token_logprobs_backward(const void* logits, int64_t st
   MCKE_RETURN_IF(check_stride(who, "logits", stride, rows, cols, false));
   MCKE_RETURN_IF(check_stride(who, "dlogits", dlogits_stride, rows, cols, true));
   const std::size_t e = dtype_bytes(dtype);
-  if (!aligned(logits, e) || !aligned(dlogits, e))
-    return fail(MCKE_INVALID_ARGUMENT, "%s: logits or dlogits is not element-aligned", who);
+  MCKE_RETURN_IF(check_aligned(who, {{"logits", logits, e}, {"dlogits", dlogits, e}, {"lse", lse, 4},
+                                     {"targets", targets, 8}, {"grad_logprobs", grad_logprobs, 4},
+                                     {"entropy", entropy, 4}, {"grad_entropy", grad_entropy, 4},
+                                     {"grad_lse", grad_lse, 4}}));
   const bool in_place = dlogits == logits && (rows == 1 || dlogits_stride == stride);
   const RowSpan outs[] = {span_of("dlogits", dlogits, rows, cols, dlogits_stride, e)};
   const RowSpan ins[] = {span_of("logits", in_place ? nullptr : logits, rows, cols, stride, e),

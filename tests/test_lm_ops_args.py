@@ -49,7 +49,10 @@ def _forward(mcke, x=A, xs=64, w=None, b=None, y=B, ys=64, mean=None, rstd=None,
     (dict(ys=63), "row stride"),
     (dict(xs=-64), "row stride"),
     (dict(xs=1 << 60), "2^40"),
-    (dict(x=A + 2), "aligned"),
+    (dict(x=A + 2), "x is not element-aligned"),
+    (dict(w=C + 2), "weight is not element-aligned"),
+    (dict(mean=C + 1), "mean is not element-aligned"),
+    (dict(rows=(1 << 31) - 1, xs=0, ys=64), "INT32_MAX"),
     (dict(y=A), "overlaps"),
     (dict(y=A + 4 * 63), "overlaps"),
     (dict(mean=A), "mean overlaps x"),
@@ -95,7 +98,8 @@ def _logprobs(mcke, x=A, stride=64, rows=4, cols=64, dtype=0, targets=B, lp=C, l
     (dict(x=None), "null"), (dict(targets=None), "null"), (dict(top=None), "null"), (dict(ids=None), "null"),
     (dict(rows=-4), "negative"), (dict(cols=0), "no columns"), (dict(dtype=1), "dtype"),
     (dict(k=-1), "top_k"), (dict(k=33), "top_k"), (dict(k=5, cols=4), "top_k"),
-    (dict(stride=-1), "row stride"), (dict(x=A + 3), "aligned"),
+    (dict(stride=-1), "row stride"), (dict(x=A + 3), "aligned"), (dict(targets=B + 4), "targets is not"),
+    (dict(cols=(1 << 22) + 1, stride=1 << 23), "top_k of more than"), (dict(ids=E + 4), "top_ids is not"),
     (dict(lp=A), "logprobs overlaps logits"), (dict(lse=C + 4), "lse overlaps logprobs"),
     (dict(ids=D), "top_ids overlaps top_logprobs"), (dict(ent=B), "entropy overlaps targets"),
 ])
@@ -166,6 +170,7 @@ def test_clip_arguments(mcke):
     _refused(mcke, l.mcke_sm100_grad_norm(p, -1, D, WS, 1 << 20, None), "negative")
     _refused(mcke, l.mcke_sm100_grad_norm(p, n, A, WS, 1 << 20, None), "overlaps")
     _refused(mcke, l.mcke_sm100_clip_grads(p, n, 1.0, A + 4, None), "overlaps")
+    _refused(mcke, l.mcke_sm100_clip_grads(p, n, 1.0, D + 2, None), "aligned")
     assert l.mcke_sm100_clip_grads(None, 0, 1.0, D, None) == mcke.OK
 
 
