@@ -714,13 +714,17 @@ void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t
 }
 
 // With alternatives a row's end is long, and blocks of four warps leave more of them on
-// an SM to cover it (8192 x 32768 bf16 with five: 115 us against 138 with eight);
-// without, blocks of eight are the faster (89 us against 94).
+// an SM to cover it (8192 x 32768 bf16 with five: 118 us against 145 with eight, 64 x
+// 131072 with eight: 12.2 against 12.9) unless the rows do not fill the device in
+// either form (one row of 131072 with twenty: 11.8 us against 10.0); without, blocks of eight
+// are the faster (89 us against 94).
 template <class T>
 void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
   const bool narrow = warp_rows<T>(rows, a.cols);
-  if (a.top_k > 0) narrow ? launch_forward<T, 1, true>(x, a, rows, s) : launch_forward<T, 4, true>(x, a, rows, s);
-  else narrow ? launch_forward<T, 1, false>(x, a, rows, s) : launch_forward<T, 8, false>(x, a, rows, s);
+  if (a.top_k == 0) narrow ? launch_forward<T, 1, false>(x, a, rows, s) : launch_forward<T, 8, false>(x, a, rows, s);
+  else if (narrow) launch_forward<T, 1, true>(x, a, rows, s);
+  else if (rows * kMaxCluster <= 148) launch_forward<T, 8, true>(x, a, rows, s);
+  else launch_forward<T, 4, true>(x, a, rows, s);
 }
 
 template <class T>

@@ -699,19 +699,23 @@ def _grad_list(grads, outs) -> bytes:
     if len(outs) != len(grads):
         raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
     index, fields = grads[0].get_device(), []
-    for kind, tensors in (("gradient", grads),) if outs is grads else (("gradient", grads), ("output", outs)):
-        for i, t in enumerate(tensors):
-            if index < 0 or t.get_device() != index or t.dtype not in _DTYPE_OF or not t.is_contiguous():
-                raise ValueError(f"{kind} {i} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
+
+    def code(t, kind, i):
+        d = _DTYPE_OF.get(t.dtype)
+        if d is None or index < 0 or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"{kind} {i} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
+        return d
+
     if outs is grads:
-        for g in grads:
-            p, d = g.data_ptr(), _DTYPE_OF[g.dtype]
+        for i, g in enumerate(grads):
+            p, d = g.data_ptr(), code(g, "gradient", i)
             fields += (p, p, g.numel(), d, d)
     else:
         for i, (g, o) in enumerate(zip(grads, outs)):
+            d, e = code(g, "gradient", i), code(o, "output", i)
             if g.shape != o.shape:
                 raise ValueError(f"output {i} must have shape {tuple(g.shape)}, got {tuple(o.shape)}")
-            fields += (g.data_ptr(), o.data_ptr(), g.numel(), _DTYPE_OF[g.dtype], _DTYPE_OF[o.dtype])
+            fields += (g.data_ptr(), o.data_ptr(), g.numel(), d, e)
     return struct.pack(_GRAD_FORMAT * len(grads), *fields)
 
 
