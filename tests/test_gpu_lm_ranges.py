@@ -1,0 +1,162 @@
+"""The language-model operators over the rest of their ranges: every kernel that a
+size chooses (rows over clusters of blocks, rows to a warp, rows by the element),
+offsets past 32 bits, very many rows, and those kernels in captured graphs and on
+several streams at once.  Oracles and tolerances are those of the operators' own
+tests."""
+from __future__ import annotations
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():  # pragma: no cover - CPU container
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+import mcke  # noqa: E402
+import test_gpu_grad_norm as gn  # noqa: E402
+import test_gpu_layer_norm as ln  # noqa: E402
+import test_gpu_token_logprobs as lp  # noqa: E402
+
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, cols", [(593, 8), (2000, 512), (1201, 520), (900, 1544), (1000, 2048), (777, 2056), (640, 4096),
+                                        (600, 5128), (999, 6144), (595, 8192), (601, 8200), (777, 12288), (650, 16384),
+                                        (600, 20000), (613, 24576), (594, 32768), (600, 8193), (1300, 4097), (700, 127),
+                                        (600, 40000)])
+def test_layer_norm_of_many_rows(rows, cols, dtype):
+    x, w, b, dy = ln._inputs(rows, cols, dtype, seed=rows)
+    y, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    ln._check_forward(x, w, b, y, mean, rstd)
+    again, _, _ = mcke.layer_norm(x, w, b, save_stats=True)
+    assert torch.equal(y, again)
+    dx, dw, db = mcke.layer_norm_backward(dy, x, mean, rstd, w)
+    ln._check_backward(x, w, mean, rstd, dy, dx, dw, db)
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), mcke.layer_norm_backward(dy, x, mean, rstd, w)))
+    mcke.check_device_errors()  # no wait of the posted sums ran out
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, cols, k", [(18, 200000, 32), (19, 200000, 32), (74, 131072, 9), (149, 70001, 8),
+                                           (1184, 2048, 5), (1183, 2048, 5), (1500, 4096, 32), (1500, 4104, 32),
+                                           (3000, 24, 20), (888, 40000, 0), (889, 40000, 1), (2, 1 << 22, 4)])
+def test_token_logprobs_by_size(rows, cols, k, dtype):
+    x, t = lp._logits(rows, cols, dtype, seed=rows + k, masked=0.02)
+    t[1::7] = -5
+    r = mcke.token_logprobs(x, t, top_k=k, entropy=True)
+    lp._check(x, t, r, k)
+    gl, ge = torch.randn(2, rows, device=DEV).unbind(0)
+    dx = mcke.token_logprobs_backward(x, r.lse, t, gl, r.entropy, ge)
+    lp._check_backward(x, t, r.lse, r.entropy, gl, ge, None, dx)
+
+
+def test_offsets_past_32_bits():
+    stride = (1 << 31) + 24
+    buf = torch.empty(2 * stride, dtype=BF16, device=DEV)
+    for cols in (4096, 4097, 16384):
+        view = torch.as_strided(buf, (2, cols), (stride, 1))
+        x, w, b, dy = ln._inputs(2, cols, BF16, seed=cols)
+        view.copy_(x)
+        y, mean, rstd = mcke.layer_norm(view, w, b, save_stats=True)
+        ln._check_forward(x, w, b, y, mean, rstd)
+        out = torch.as_strided(buf, (2, cols), (stride, 1), 1 << 20)
+        mcke.layer_norm_backward(dy, view, mean, rstd, w, out=out)
+        assert torch.equal(out, mcke.layer_norm_backward(dy, x, mean, rstd, w)[0])
+        t = torch.tensor([3, cols - 1], device=DEV)
+        r = mcke.token_logprobs(view, t, top_k=3, entropy=True)
+        lp._check(x, t, r, 3)
+        g = torch.ones(2, device=DEV)
+        want = mcke.token_logprobs_backward(x, r.lse, t, g)
+        assert torch.equal(mcke.token_logprobs_backward(view, r.lse, t, g, out=out), want)
+        assert torch.equal(mcke.token_logprobs_backward(view, r.lse, t, g, out=view), want)
+    # one tensor of more than 2^31 elements
+    buf.zero_()
+    buf[-1] = 3.0
+    buf[5] = 4.0
+    assert mcke.grad_norm([buf]) == 5.0
+    mcke.clip_grad_norm([buf], 2.5)
+    assert buf[-1] == 1.5 and buf[5] == 2.0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_very_many_rows(dtype):
+    rows = 300007
+    x, w, b, dy = ln._inputs(rows, 16, dtype, seed=2)
+    y, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    ln._check_forward(x, w, b, y, mean, rstd)
+    ln._check_backward(x, w, mean, rstd, dy, *mcke.layer_norm_backward(dy, x, mean, rstd, w))
+    t = torch.randint(0, 16, (rows,), device=DEV)
+    r = mcke.token_logprobs(x, t, top_k=2, entropy=True)
+    lp._check(x, t, r, 2)
+    g = torch.randn(rows, device=DEV)
+    lp._check_backward(x, t, r.lse, None, g, None, None, mcke.token_logprobs_backward(x, r.lse, t, g))
+
+
+def _wide(seed):
+    """Calls that run over clusters of blocks and with alternatives."""
+    x, w, b, dy = ln._inputs(600, 16384, BF16, seed=seed)
+    z, t = lp._logits(3, 100000, BF16, seed=seed)
+    grads = gn._grads([3000001, 17, 70000], [F32, BF16], seed=seed)
+    outs = [torch.empty_like(g) for g in grads]
+
+    def run(stream=None):
+        y, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True, stream=stream)
+        dx, dw, db = mcke.layer_norm_backward(dy, x, mean, rstd, w, stream=stream)
+        r = mcke.token_logprobs(z, t, top_k=20, entropy=True, stream=stream)
+        n = mcke.clip_grad_norm(grads, 0.1, out=outs, stream=stream)
+        return [y, mean, rstd, dx, dw, db, *r, n, *outs]
+
+    return run
+
+
+def test_wide_calls_captured_and_at_once():
+    calls = [_wide(s) for s in (1, 2, 3)]
+    want = [[v.clone() for v in c()] for c in calls]
+    torch.cuda.synchronize()
+    graphs, got = [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got.append(c())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    del graphs
+    eager = []
+    for _ in range(3):
+        eager = [c(stream=s) for c, s in zip(calls, streams)]
+    torch.cuda.synchronize()
+    for a, b in zip(eager, want):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
+    mcke.check_device_errors()
+    # the default stream by its handle
+    with torch.cuda.stream(streams[0]):
+        out = calls[0](stream=0)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(out, want[0]))
+
+
+def test_a_workspace_of_the_callers():
+    x, w, b, dy = ln._inputs(700, 1024, BF16, seed=9)
+    _, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    want = mcke.layer_norm_backward(dy, x, mean, rstd, w)
+    ws = torch.full((mcke.layer_norm_backward_workspace_bytes(700, 1024),), 255, dtype=torch.uint8, device=DEV)  # NaNs
+    got = mcke.layer_norm_backward(dy, x, mean, rstd, w, workspace=ws)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(mcke.MckeError, match="workspace"):
+        mcke.layer_norm_backward(dy, x, mean, rstd, w, workspace=ws[:64])
+    grads = [x, w]
+    ws = torch.full((mcke.grad_norm_workspace_bytes(2),), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(mcke.grad_norm(grads, workspace=ws), mcke.grad_norm(grads))
+    out = torch.zeros((), device=DEV)
+    assert mcke.grad_norm(grads, norm=out) is out and out > 0
