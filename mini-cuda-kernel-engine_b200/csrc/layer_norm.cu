@@ -1121,32 +1121,50 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 // dw and db from the slabs' partial sums [slabs][2 cols]; zeros for no slab.  A block
-// folds 32 columns: warp w adds slabs w, w + 32, ... in order, all of them in flight at
-// once, then the warps are added in order.
+// folds 32 kPer columns: warp w adds slabs w, w + 32, ... in order, all of them in flight
+// at once, then the warps' sums are added in a fixed tree.  kPer = 4, for wide rows:
+// fewer blocks than fit at once (4096 x 16384 bf16, both kernels: 71.5 us with 1, 69.7 with 4).
 constexpr int kFoldWarps = 32;
+template <int kPer>
 __global__ void __launch_bounds__(32 * kFoldWarps)
     layer_norm_fold_kernel(const float* __restrict__ part, int slabs, float* __restrict__ dweight,
                            float* __restrict__ dbias, int cols) {
   pdl_entry();
-  __shared__ float red[kFoldWarps][33];
+  __shared__ float red[kPer][kFoldWarps][33];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t width = 2 * static_cast<int64_t>(cols), c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
-  float s = 0.0f;
+  const int64_t width = 2 * static_cast<int64_t>(cols);
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * 32 * kPer, c = first + lane * kPer;
+  float s[kPer] = {};
   if (c < width) {
 #pragma unroll
-    for (int k = 0; k < (kStreamBlocks + kFoldWarps - 1) / kFoldWarps; ++k)
-      if (warp + k * kFoldWarps < slabs) s += part[(warp + k * kFoldWarps) * width + c];
+    for (int k = 0; k < (kStreamBlocks + kFoldWarps - 1) / kFoldWarps; ++k) {
+      if (warp + k * kFoldWarps >= slabs) break;
+      const float* p = part + (warp + k * kFoldWarps) * width + c;
+      if constexpr (kPer == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(p);
+        s[0] += v.x;
+        s[1] += v.y;
+        s[2] += v.z;
+        s[3] += v.w;
+      } else {
+        s[0] += *p;
+      }
+    }
   }
-  red[warp][lane] = s;
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) red[j][warp][lane] = s[j];
   __syncthreads();
-  // warp w sums up column w of the 32, a lane per warp's share
-  const int64_t mine = static_cast<int64_t>(blockIdx.x) * 32 + warp;
-  s = warp_all_sum(red[lane][warp]);
-  if (lane > 0 || mine >= width) return;
-  if (mine < cols) {
-    if (dweight) dweight[mine] = s;
-  } else if (dbias) {
-    dbias[mine - cols] = s;
+  // warp w sums up columns kPer w and on, a lane per warp's share
+#pragma unroll
+  for (int j = 0; j < kPer; ++j) {
+    const float sum = warp_all_sum(red[j][lane][warp]);
+    const int64_t mine = first + warp * kPer + j;
+    if (lane > 0 || mine >= width) continue;
+    if (mine < cols) {
+      if (dweight) dweight[mine] = sum;
+    } else if (dbias) {
+      dbias[mine - cols] = sum;
+    }
   }
 }
 
@@ -1362,9 +1380,14 @@ void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* d
                    static_cast<int64_t>(a.cols));
     }
   }
-  if (dweight || dbias)
-    launch_async(layer_norm_fold_kernel, static_cast<unsigned>((2 * static_cast<int64_t>(a.cols) + 31) / 32),
-                 32 * kFoldWarps, 0, s, static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
+  if (!dweight && !dbias) return;
+  const int64_t width = 2 * static_cast<int64_t>(a.cols);
+  if (a.cols >= 8192 && width % 4 == 0)
+    launch_async(layer_norm_fold_kernel<4>, static_cast<unsigned>((width + 127) / 128), 32 * kFoldWarps, 0, s,
+                 static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
+  else
+    launch_async(layer_norm_fold_kernel<1>, static_cast<unsigned>((width + 31) / 32), 32 * kFoldWarps, 0, s,
+                 static_cast<const float*>(a.part), static_cast<int>(slabs), dweight, dbias, a.cols);
 }
 
 }  // namespace
