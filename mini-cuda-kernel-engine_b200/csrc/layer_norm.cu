@@ -34,15 +34,6 @@ template <>
 struct Unit<float> {
   static constexpr int kPer = 4;
   static __device__ __forceinline__ uint4 load(const float* p) { return ld_stream_u4(p); }
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[4]) {
-    v[0] = __uint_as_float(q.x);
-    v[1] = __uint_as_float(q.y);
-    v[2] = __uint_as_float(q.z);
-    v[3] = __uint_as_float(q.w);
-  }
-  static __device__ __forceinline__ void store(float* p, const float (&v)[4]) {
-    st_stream_f4(p, make_float4(v[0], v[1], v[2], v[3]));
-  }
   static __device__ __forceinline__ void pairs(const uint4& q, F2 (&v)[2]) {
     v[0] = f2(__uint_as_float(q.x), __uint_as_float(q.y));
     v[1] = f2(__uint_as_float(q.z), __uint_as_float(q.w));
@@ -56,18 +47,6 @@ template <>
 struct Unit<uint16_t> {
   static constexpr int kPer = 8;
   static __device__ __forceinline__ uint4 load(const uint16_t* p) { return ld_stream_u4(p); }
-  static __device__ __forceinline__ void unpack(const uint4& q, float (&v)[8]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[2 * j] = bf16_lo(w[j]);
-      v[2 * j + 1] = bf16_hi(w[j]);
-    }
-  }
-  static __device__ __forceinline__ void store(uint16_t* p, const float (&v)[8]) {
-    st_stream_u4(p, make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                               pack_bf16x2(v[6], v[7])));
-  }
   static __device__ __forceinline__ void pairs(const uint4& q, F2 (&v)[4]) {
     const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
@@ -136,8 +115,8 @@ __device__ __forceinline__ void load_param_pairs(const float* p, int c, float ot
 
 // A row in the registers of kRowWarps warps, kUnits units a thread (a warp per row: eight
 // rows a block, no barrier; else a block per row): x is read once and y
-// written once.  The units stay packed, so a bf16 row of 4096 is 64 registers of
-// one warp.  kFull: the row fills the threads' units, and none needs a check.
+// written once.  kFull: the row fills the threads' units, and none needs a check.
+// Bound by HBM for f32: 16384 x 2048 in 42.3 us (6.35 TB/s, 0.97 of the copy rate).
 template <class T, int kUnits, int kRowWarps, bool kFull>
 __global__ void __launch_bounds__(kRowWarps == 1 ? kThreads : 32 * kRowWarps, RowBlocks<T, kUnits, kRowWarps>::kMin)
     layer_norm_kernel(const ForwardArgs a) {
@@ -339,7 +318,10 @@ __device__ __forceinline__ void group_all_sum(float (&v)[4], GroupSums<kW>& red,
 // Two rows at a time, 16 elements of each to a thread; the sums of the next two
 // rows and the squared deviations of the current two are reduced together, so
 // two rows cost one barrier and six shuffles although each variance is taken
-// about its row's exact mean.
+// about its row's exact mean.  bf16 rows have half the bytes to cover the same
+// instructions: 8192 x 4096 bf16 took 48 us with a row to a block and the parameters
+// from L1, 29.5 with one row at a time here, 22.4 with two (5.99 TB/s, 0.92 of the copy
+// rate); 32768 x 1024 20.6 us (1.00).
 template <class T, int kW, int kGroups, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel(const ForwardArgs a) {
   pdl_entry();
@@ -584,11 +566,13 @@ __device__ __forceinline__ void collect_sums(float (&v)[kN], PostedSums<kN, kW, 
   for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
 }
 
-// Rows over the blocks of a cluster.  The statistics take two exchanges, the mean's and that of the squared deviations
-// about it, and both ride in one post: turn p collects what turn p - 1 posted (the
-// means of rows p, the variances of rows p - 1), posts the sums of rows p + 1 and
-// the squared deviations of rows p, and writes rows p - 1 while they arrive.  "Rows
-// p" are kRows rows; each is read from the ring in three turns running.
+// Rows over the blocks of a cluster.  The statistics take two exchanges, the mean's and
+// that of the squared deviations about it, and both ride in one post: turn p collects
+// what turn p - 1 posted (the means of rows p, the variances of rows p - 1), posts the
+// sums of rows p + 1 and the squared deviations of rows p, and writes rows p - 1 while
+// they arrive.  "Rows p" are kRows rows; each is read from the ring in three turns
+// running.  4096 x 16384 bf16 43.6 us (6.16 TB/s, 0.94 of the copy rate); for rows that one
+// block holds the kernel above is the faster (8192 x 4096: 22.4 us against 24.4).
 template <class T, int kW, int kCluster, int kRows, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const ForwardArgs a) {
   pdl_entry();
@@ -769,6 +753,11 @@ __device__ __forceinline__ bool join_groups(F2* cell, int group, F2* dw, F2* db)
 // block's groups are added in shared memory at the end.  Each turn of the loop
 // posts the sums of kRows rows and writes dx of the rows of the turn before, whose
 // units are read a second time from the ring.
+//
+// f32 is bound by HBM (16384 x 2048 64 us, 0.96 of the copy rate), bf16 by what is issued
+// for its elements: 8192 x 4096 51 us with a barrier a row, 44 with the sums posted, 36.5
+// with two rows a turn, 35.4 (5.69 TB/s, 0.87) with the ring on 128 bytes.  24 warps
+// instead of 16 spill (49 us).  4096 x 16384 over pairs of blocks 69.7 us (0.89).
 template <class T, int kW, int kGroups, int kCluster, int kRows, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kernel(const BackwardArgs a) {
   pdl_entry();
@@ -929,7 +918,9 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
 // The same for rows that are not whole 16-byte units: consecutive threads have consecutive
 // elements, 16 of them in pairs (of columns c and c + kTpg).  Elements of the row after
 // next come into registers (two bytes are less than an asynchronous copy moves) and go
-// to the ring, of the last row, this one and the next, a turn later.
+// to the ring, of the last row, this one and the next, a turn later.  Bound by the
+// element-wide accesses: 8192 x 4097 bf16 99 us (0.31 of the copy rate; a pass each for dx and
+// for the sums took 142), 5003 x 1537 f32 26 us (0.54).
 template <class T, int kW, int kGroups>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elements_kernel(const BackwardArgs a) {
   pdl_entry();
@@ -1040,7 +1031,7 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
   }
 }
 
-// Rows of any length: one block per row, three reads of it.
+// Rows of any length: one block per row, three reads of it (the second and third from L2).
 template <class T>
 __global__ void __launch_bounds__(kThreads)
     layer_norm_row_kernel(const T* __restrict__ x, int64_t x_stride, const float* __restrict__ weight,
@@ -1283,6 +1274,14 @@ void launch_forward_stream(const ForwardArgs& a, cudaStream_t s) {
   });
 }
 
+// Which kernel, with kernel times of both sides (us):
+//   whole units, few rows   a row to 1, 4 or 16 warps, one unit to a thread where it fits:
+//                           1000 x 1024 f32 2.5, streamed 3.1
+//   f32 up to 8192 columns  a row to 1, 2 or 4 warps: 16384 x 2048 42.3, streamed 47.9
+//   bf16, and wider f32     streamed: 8192 x 4096 bf16 22.4, a row to a warp 37.5; over
+//                           clusters: 4096 x 16384 bf16 43.6, a row to a block 99
+//   the rest up to 16384    element by element: 8192 x 4097 bf16 46, three reads 94
+//   wider still             three reads
 template <class T>
 void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
   using std::integral_constant;

@@ -399,7 +399,10 @@ __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t 
 // block's shared memory, in order.  kRowWarps = 1: a row to each warp, four to a block.
 //
 // One read of the row: a warp has kLoads chunks in flight, takes their maximum, and
-// adds up the sums on its scale.
+// adds up the sums on its scale.  f32 is bound by HBM (4096 x 32768 80 us, 6.7 TB/s, 1.02 of
+// the copy rate: reads alone), bf16 by issue, the exponential unit 65% busy (8192 x
+// 32768 88.9 us, 6.04 TB/s, 0.92); with alternatives by a row's end, in which most warps
+// wait (the same rows with five 118 us).  One row of 131072: 10 us, of which 2 read it.
 template <int kRowWarps>
 constexpr int kBlockWarps = kRowWarps == 1 ? 4 : kRowWarps;
 
@@ -571,6 +574,9 @@ struct Grads {
 };
 
 // dx may be x itself: a vector is read before it is written, by the same thread.
+// Bound by HBM: 4096 x 50257 bf16 with the entropy's gradient 136 us (6.04 TB/s, 0.92 of the copy
+// rate), 2048 x 32768 f32 80 us (1.02).  A check for whole blocks of vectors costs more in
+// registers than it saves (144 us).
 // `threads` threads of a block (a power of two) take a part of a row, kVecs vectors
 // each; kSame: dx has the row's offset from a 16-byte boundary, so whole vectors
 // are stored.
