@@ -574,12 +574,12 @@ struct Grads {
 };
 
 // dx may be x itself: a vector is read before it is written, by the same thread.
-// Bound by HBM: 4096 x 50257 bf16 with the entropy's gradient 136 us (6.04 TB/s, 0.92 of the copy
-// rate), 2048 x 32768 f32 80 us (1.02).  A check for whole blocks of vectors costs more in
-// registers than it saves (144 us).
 // `threads` threads of a block (a power of two) take a part of a row, kVecs vectors
 // each; kSame: dx has the row's offset from a 16-byte boundary, so whole vectors
 // are stored.
+// Bound by HBM: 4096 x 50257 bf16 with the entropy's gradient 136 us (6.04 TB/s, 0.92 of
+// the copy rate), 2048 x 32768 f32 80 us (1.02).  A check for whole blocks of vectors costs
+// more in registers than it saves (144 us).
 constexpr int kVecs = 4;
 template <class T, bool kEntropy, bool kSame>
 __global__ void __launch_bounds__(kThreads, 6)
