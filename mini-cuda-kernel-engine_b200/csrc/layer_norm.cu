@@ -915,44 +915,84 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
   }
 }
 
+// 16 elements of a thread, one behind the other, as units.
+__device__ __forceinline__ void pack_units(const float (&e)[16], uint4 (&q)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    q[i] = make_uint4(__float_as_uint(e[4 * i]), __float_as_uint(e[4 * i + 1]), __float_as_uint(e[4 * i + 2]),
+                      __float_as_uint(e[4 * i + 3]));
+}
+__device__ __forceinline__ void pack_units(const uint16_t (&e)[16], uint4 (&q)[2]) {
+  auto word = [&](int j) { return static_cast<uint32_t>(e[2 * j]) | static_cast<uint32_t>(e[2 * j + 1]) << 16; };
+#pragma unroll
+  for (int i = 0; i < 2; ++i) q[i] = make_uint4(word(4 * i), word(4 * i + 1), word(4 * i + 2), word(4 * i + 3));
+}
+
 // The same for rows that are not whole 16-byte units: consecutive threads have consecutive
-// elements, 16 of them in pairs (of columns c and c + kTpg).  Elements of the row after
-// next come into registers (two bytes are less than an asynchronous copy moves) and go
-// to the ring, of the last row, this one and the next, a turn later.  Bound by the
-// element-wide accesses: 8192 x 4097 bf16 99 us (0.31 of the copy rate; a pass each for dx and
-// for the sums took 142), 5003 x 1537 f32 26 us (0.54).
-template <class T, int kW, int kGroups>
+// elements, 16 of them each, in pairs (of columns c and c + kTpr).  Elements of the row
+// after next come into registers (two bytes are less than an asynchronous copy
+// moves) and go to the ring, of the last row, this one and the next, a turn later, as
+// units: a thread reads only its own.  Bound by the element-wide accesses: 8192 x 4097
+// bf16 85 us (2.37 TB/s, 0.36 of the copy rate; 98 with elements in the ring, 142 with a pass
+// each for dx and for the sums), 5003 x 1537 f32 26 us (0.54); over clusters 2000 x 20001 bf16
+// 119 us, the two passes 195.
+template <class T, int kW, int kGroups, int kCluster>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elements_kernel(const BackwardArgs a) {
   pdl_entry();
-  constexpr int kPairs = 8, kTpg = 32 * kW, kThr = kTpg * kGroups, kStages = 3;
-  extern __shared__ __align__(128) uint4 ring[];  // T [stage][dy, x][element][thread]
-  __shared__ PostedSums<2, kW, 1> posted[kGroups];
-  const int group = threadIdx.x / kTpg, t = threadIdx.x % kTpg;
-  auto col = [&](int e) { return e * kTpg + t; };
-  const int step = gridDim.x * kGroups;
-  int row = blockIdx.x + gridDim.x * group;
-  if (t == 0) init_sums(posted[group]);
-  __syncthreads();
-  T* const cells = reinterpret_cast<T*>(ring) + threadIdx.x;
-  auto cell = [&](int stage, int operand, int e) { return cells + ((stage * 2 + operand) * 2 * kPairs + e) * kThr; };
-  T dyr[2 * kPairs], xr[2 * kPairs];
+  using U = Unit<T>;
+  constexpr int kPer = U::kPer, kUnits = 16 / kPer, kPairs = 8, kStages = 3;
+  constexpr int kTpg = 32 * kW, kThr = kTpg * kGroups, kTpr = kTpg * kCluster;
+  extern __shared__ __align__(128) uint4 ring[];  // [stage][dy, x][unit][thread]
+  __shared__ PostedSums<2, kW, kCluster> posted[kGroups];
+  static_assert(kGroups == 1 || kCluster == 1, "a block of a cluster is one group");
+  const int group = threadIdx.x / kTpg;
+  const int t = threadIdx.x % kTpg + (kCluster > 1 ? static_cast<int>(block_in_cluster()) * kTpg : 0);
+  auto col = [&](int e) { return e * kTpr + t; };
+  const int clusters = gridDim.x / kCluster, cluster = blockIdx.x / kCluster;
+  const int step = clusters * kGroups;
+  int row = cluster + clusters * group;
+  if (threadIdx.x % kTpg == 0) init_sums(posted[group]);
+  if constexpr (kCluster > 1) {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    cluster_barrier();  // every block of it runs, its barriers in place, before one posts into another
+  } else {
+    __syncthreads();
+  }
+  uint4* const units = ring + threadIdx.x;
+  auto unit = [&](int stage, int operand, int i) { return units + ((stage * 2 + operand) * kUnits + i) * kThr; };
+  T dyr[16], xr[16];
   auto load = [&](int64_t r) {
     if (r >= a.rows) return;
     const T* dy = static_cast<const T*>(a.dy) + r * a.dy_stride;
     const T* x = static_cast<const T*>(a.x) + r * a.x_stride;
 #pragma unroll
-    for (int e = 0; e < 2 * kPairs; ++e) {
+    for (int e = 0; e < 16; ++e) {
       dyr[e] = col(e) < a.cols ? __ldg(dy + col(e)) : T(0);
       xr[e] = col(e) < a.cols ? __ldg(x + col(e)) : T(0);
     }
   };
   auto store = [&](int stage) {
+    uint4 q[2][kUnits];
+    pack_units(dyr, q[0]);
+    pack_units(xr, q[1]);
 #pragma unroll
-    for (int e = 0; e < 2 * kPairs; ++e) {
-      *cell(stage, 0, e) = dyr[e];
-      *cell(stage, 1, e) = xr[e];
+    for (int i = 0; i < kUnits; ++i) {
+      *unit(stage, 0, i) = q[0][i];
+      *unit(stage, 1, i) = q[1][i];
     }
   };
+  // f(first pair, dy, x) over this thread's units of a stage
+  auto for_units = [&](int stage, auto&& f) {
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      F2 d[kPer / 2], v[kPer / 2];
+      U::pairs(*unit(stage, 0, i), d);
+      U::pairs(*unit(stage, 1, i), v);
+      f(i * (kPer / 2), d, v);
+    }
+  };
+#pragma unroll
+  for (int e = 0; e < 16; ++e) dyr[e] = xr[e] = T(0);
   load(row);
   F2 w[kPairs], dw[kPairs], db[kPairs];
 #pragma unroll
@@ -962,7 +1002,7 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
     dw[i] = db[i] = f2(0.0f);
   }
   store(0);
-  load(row + step);
+  load(static_cast<int64_t>(row) + step);
   const float n = static_cast<float>(a.cols), inv_n = 1.0f / n;
   auto mean_of = [&](int r) { return r < a.rows ? __ldg(a.mean + r) : 0.0f; };
   auto rstd_of = [&](int r) { return r < a.rows ? __ldg(a.rstd + r) : 0.0f; };
@@ -973,17 +1013,17 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
     if (row < a.rows) {
       const F2 minus_mu = f2(-mu), rr = f2(r);
       F2 s1 = f2(0.0f), s2 = f2(0.0f);
+      for_units(stage, [&](int i, const auto& d, const auto& v) {
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        // columns past the row have dy = 0 and add nothing
-        const F2 d = f2(ld_val(cell(stage, 0, 2 * i)), ld_val(cell(stage, 0, 2 * i + 1)));
-        const F2 v = f2(ld_val(cell(stage, 1, 2 * i)), ld_val(cell(stage, 1, 2 * i + 1)));
-        const F2 p = mul2(d, add2(v, minus_mu));
-        db[i] = add2(db[i], d);
-        dw[i] = fma2(p, rr, dw[i]);
-        s1 = fma2(d, w[i], s1);
-        s2 = fma2(p, w[i], s2);
-      }
+        for (int j = 0; j < kPer / 2; ++j) {
+          // columns past the row have dy = 0 and add nothing
+          const F2 p = mul2(d[j], add2(v[j], minus_mu));
+          db[i + j] = add2(db[i + j], d[j]);
+          dw[i + j] = fma2(p, rr, dw[i + j]);
+          s1 = fma2(d[j], w[i + j], s1);
+          s2 = fma2(p, w[i + j], s2);
+        }
+      });
       const float sums[2] = {sum2(s1), sum2(s2)};
       post_sums(sums, posted[group], turn % kPlaces);
     }
@@ -995,15 +1035,14 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
       const F2 k1 = f2(-last_r * div_by(c[0], n, inv_n));
       const F2 k2 = f2(-last_r * last_r * (last_r * div_by(c[1], n, inv_n)));
       T* dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row - step) * a.dx_stride;
+      for_units(last_stage, [&](int i, const auto& d, const auto& v) {
 #pragma unroll
-      for (int i = 0; i < kPairs; ++i) {
-        if (col(2 * i) >= a.cols) break;
-        const F2 d = f2(ld_val(cell(last_stage, 0, 2 * i)), ld_val(cell(last_stage, 0, 2 * i + 1)));
-        const F2 v = f2(ld_val(cell(last_stage, 1, 2 * i)), ld_val(cell(last_stage, 1, 2 * i + 1)));
-        const float2 g = split(fma2(add2(v, minus_mu), k2, fma2(mul2(d, w[i]), rr, k1)));
-        st_val(dx + col(2 * i), g.x);
-        if (col(2 * i + 1) < a.cols) st_val(dx + col(2 * i + 1), g.y);
-      }
+        for (int j = 0; j < kPer / 2; ++j) {
+          const float2 g = split(fma2(add2(v[j], minus_mu), k2, fma2(mul2(d[j], w[i + j]), rr, k1)));
+          if (col(2 * (i + j)) < a.cols) st_val(dx + col(2 * (i + j)), g.x);
+          if (col(2 * (i + j) + 1) < a.cols) st_val(dx + col(2 * (i + j) + 1), g.y);
+        }
+      });
     }
     store(next_stage);
     load(static_cast<int64_t>(row) + 2 * step);
@@ -1014,9 +1053,10 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
     last_stage = stage;
     stage = next_stage;
   }
+  if constexpr (kCluster > 1) cluster_barrier();  // no block leaves while another's post may be on its way to it
   if (!a.part) return;
   if (!join_groups<kGroups, kTpg, kPairs>(reinterpret_cast<F2*>(ring), group, dw, db)) return;
-  float* const out = a.part + static_cast<int64_t>(blockIdx.x) * 2 * a.cols;
+  float* const out = a.part + static_cast<int64_t>(cluster) * 2 * a.cols;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i) {
     const float2 x = split(dw[i]), b = split(db[i]);
@@ -1231,7 +1271,7 @@ int64_t launch_stream(void (*kernel)(const A), const A& a, int64_t items, int th
 
 // Calls f(warps, blocks) with the smallest group, of 1 .. 16 warps in each of 1, 2 or 4
 // blocks, whose threads hold a row of `cols` <= kStreamCols at 16 elements each.
-constexpr int64_t kStreamCols = 4 * 8192, kElementCols = 8192;
+constexpr int64_t kStreamCols = 4 * 8192;
 template <class F>
 void with_group(int64_t cols, F&& f) {
   using std::integral_constant;
@@ -1356,17 +1396,15 @@ void launch_backward(const BackwardArgs& a, bool whole, float* dweight, float* d
   int64_t slabs = 0;
   if (a.rows > 0 && whole && a.cols <= kStreamCols) {
     slabs = launch_backward_stream<T>(a, s);
-  } else if (a.rows > 0 && a.cols <= kElementCols) {
+  } else if (a.rows > 0 && a.cols <= kStreamCols) {
     with_group(a.cols, [&](auto warps, auto blocks) {
-      constexpr int kW = decltype(warps)::value;
-      if constexpr (decltype(blocks)::value == 1) {
-        constexpr int kGroups = kW == 1 ? 15 : 16 / kW;
-        // the ring, or at the end the groups' sums
-        constexpr std::size_t kRing = 3 * 2 * 16 * 32 * kW * kGroups * sizeof(T);
-        constexpr std::size_t kSums = static_cast<std::size_t>(kGroups - 1) * 32 * 32 * kW * sizeof(float);
-        slabs = launch_stream<1>(layer_norm_backward_elements_kernel<T, kW, kGroups>, a, a.rows, 32 * kW * kGroups,
-                                 kRing > kSums ? kRing : kSums, s);
-      }
+      constexpr int kW = decltype(warps)::value, kC = decltype(blocks)::value;
+      constexpr int kGroups = kC > 1 ? 1 : kW == 1 ? 15 : 16 / kW;
+      // the ring, or at the end the groups' sums
+      constexpr std::size_t kRing = 3 * 2 * 16 * 32 * kW * kGroups * sizeof(T);
+      constexpr std::size_t kSums = static_cast<std::size_t>(kGroups - 1) * 32 * 32 * kW * sizeof(float);
+      slabs = launch_stream<kC>(layer_norm_backward_elements_kernel<T, kW, kGroups, kC>, a, a.rows, 32 * kW * kGroups,
+                                kRing > kSums ? kRing : kSums, s);
     });
   } else if (a.rows > 0) {
     launch_async(layer_norm_dx_kernel<T>, static_cast<unsigned>(a.rows), kThreads, 0, s, dy, a.dy_stride, x, a.x_stride,

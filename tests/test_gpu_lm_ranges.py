@@ -40,6 +40,30 @@ def test_layer_norm_of_many_rows(rows, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, cols", [(600, 8193), (601, 12289), (149, 12287), (1, 8201), (297, 16383), (600, 16385),
+                                        (299, 20001), (3, 24577), (65, 24575), (595, 32767), (40, 32769), (2, 20001)])
+def test_layer_norm_of_wide_odd_rows(rows, cols, dtype):
+    x, w, b, dy = ln._inputs(rows, cols, dtype, seed=cols)
+    y, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    ln._check_forward(x, w, b, y, mean, rstd)
+    dx, dw, db = mcke.layer_norm_backward(dy, x, mean, rstd, w)
+    ln._check_backward(x, w, mean, rstd, dy, dx, dw, db)
+    # rows of another stride: the same kernel, the same bits
+    apart = torch.full((rows, cols + 3), float("nan"), dtype=dtype, device=DEV)
+    apart[:, :cols] = x
+    out = torch.full_like(apart, 7.0)
+    again = mcke.layer_norm_backward(dy, apart[:, :cols], mean, rstd, w, out=out[:, :cols])
+    assert all(torch.equal(p, q) for p, q in zip((dx, dw, db), again))
+    assert bool((out[:, cols:] == 7.0).all())
+    # whole units that start off a 16-byte boundary
+    odd = torch.empty(rows * (cols // 8 * 8) + 1, dtype=dtype, device=DEV)[1:].view(rows, cols // 8 * 8)
+    odd.copy_(x[:, : cols // 8 * 8])
+    y, mean, rstd = mcke.layer_norm(odd, save_stats=True)
+    ln._check_forward(odd, None, None, y, mean, rstd)
+    mcke.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows, cols, k", [(18, 200000, 32), (19, 200000, 32), (74, 131072, 9), (149, 70001, 8),
                                            (1184, 2048, 5), (1183, 2048, 5), (1500, 4096, 32), (1500, 4104, 32),
                                            (3000, 24, 20), (888, 40000, 0), (889, 40000, 1), (2, 1 << 22, 4)])
