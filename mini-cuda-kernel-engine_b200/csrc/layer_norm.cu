@@ -393,16 +393,16 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       sums[k] = take(row + step + k, stage, k, next[k]);
-      const F2 minus_mu = f2(-mu[k]);
       F2 d2 = f2(0.0f);
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
+        const F2 minus_mu = f2(live(i) ? -mu[k] : 0.0f);  // a deviation of 0 past the row's end
         F2 v[kPairs];
         U::pairs(q[k][i], v);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) {
           const F2 d = add2(v[j], minus_mu);
-          if (live(i)) d2 = fma2(d, d, d2);
+          d2 = fma2(d, d, d2);
         }
       }
       sums[2 + k] = sum2(d2);
@@ -419,12 +419,11 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_stream_kernel
       const F2 rr = f2(r), minus_mu = f2(-mu[k]);
 #pragma unroll
       for (int i = 0; i < kUnits; ++i) {
-        if (!live(i)) continue;
         F2 v[kPairs];
         U::pairs(q[k][i], v);
 #pragma unroll
         for (int j = 0; j < kPairs; ++j) v[j] = fma2(mul2(add2(v[j], minus_mu), rr), w[i][j], b[i][j]);
-        U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
+        if (live(i)) U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
       }
     }
     yr += step * a.y_stride;
@@ -571,13 +570,14 @@ __device__ __forceinline__ void collect_sums(float (&v)[kN], PostedSums<kN, kW, 
 // what turn p - 1 posted (the means of rows p, the variances of rows p - 1), posts the
 // sums of rows p + 1 and the squared deviations of rows p, and writes rows p - 1 while
 // they arrive.  "Rows p" are kRows rows; each is read from the ring in three turns
-// running.  4096 x 16384 bf16 43.6 us (6.16 TB/s, 0.94 of the copy rate); for rows that one
-// block holds the kernel above is the faster (8192 x 4096: 22.4 us against 24.4).
-template <class T, int kW, int kCluster, int kRows, int kStages, bool kFull>
+// running; kElems elements to a thread.  4096 x 16384 bf16 43.6 us (6.16 TB/s, 0.94 of the
+// copy rate); for rows that one block holds the kernel above is the faster (8192 x 4096:
+// 22.4 us against 24.4).
+template <class T, int kElems, int kW, int kCluster, int kRows, int kStages, bool kFull>
 __global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const ForwardArgs a) {
   pdl_entry();
   using U = Unit<T>;
-  constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = 16 / kPer;
+  constexpr int kPer = U::kPer, kPairs = kPer / 2, kUnits = kElems / kPer;
   using S = Stream<T, kUnits, kW, 1, kStages, kRows>;
   extern __shared__ __align__(128) uint4 ring[];
   __shared__ PostedSums<2 * kRows, kW, kCluster> posted;
@@ -649,20 +649,18 @@ __global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const Fo
         if (row + step + k < a.rows) {
 #pragma unroll
           for (int i = 0; i < kUnits; ++i) {
-            if (!live(i)) continue;
             F2 v[kPairs];
-            U::pairs(*slot(next_stage, k, i), v);
+            U::pairs(live(i) ? *slot(next_stage, k, i) : no_unit(), v);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) s = add2(s, v[j]);
           }
         }
         if (turn > 0 && row + k < a.rows) {
-          const F2 minus_mu = f2(-mu[k]);
 #pragma unroll
           for (int i = 0; i < kUnits; ++i) {
-            if (!live(i)) continue;
+            const F2 minus_mu = f2(live(i) ? -mu[k] : 0.0f);  // a deviation of 0 past the row's end
             F2 v[kPairs];
-            U::pairs(*slot(stage, k, i), v);
+            U::pairs(live(i) ? *slot(stage, k, i) : no_unit(), v);
 #pragma unroll
             for (int j = 0; j < kPairs; ++j) {
               const F2 d = add2(v[j], minus_mu);
@@ -688,12 +686,11 @@ __global__ void __launch_bounds__(32 * kW, 1) layer_norm_cluster_kernel(const Fo
         const F2 rr = f2(r), minus_mu = f2(-last_mu[k]);
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-          if (!live(i)) continue;
           F2 v[kPairs];
-          U::pairs(*slot(last_stage, k, i), v);
+          U::pairs(live(i) ? *slot(last_stage, k, i) : no_unit(), v);
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) v[j] = fma2(mul2(add2(v[j], minus_mu), rr), w[i][j], b[i][j]);
-          U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
+          if (live(i)) U::store_pairs(yr + k * a.y_stride + i * kTpr * kPer, v);
         }
       }
       yr += step * a.y_stride;
@@ -845,10 +842,12 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
         F2 s1 = f2(0.0f), s2 = f2(0.0f);
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-          if (!live(i) || (kRows > 1 && row + k >= a.rows)) continue;
+          // past the row's end, and in a row that is not there, dy = 0 adds nothing; no branch
+          // around a unit's work (1600 x 20000 bf16: 47.6 us, with one 50.0)
+          const bool there = live(i) && (kRows == 1 || row + k < a.rows);
           F2 d[kPairs], v[kPairs];
-          U::pairs(*slot(stage, k, 0, i), d);
-          U::pairs(*slot(stage, k, 1, i), v);
+          U::pairs(there ? *slot(stage, k, 0, i) : no_unit(), d);
+          U::pairs(there ? *slot(stage, k, 1, i) : no_unit(), v);
 #pragma unroll
           for (int j = 0; j < kPairs; ++j) {
             const F2 dev = add2(v[j], minus_mu), p = mul2(d[j], dev);
@@ -875,14 +874,13 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
         const F2 k2 = f2(-last_r[k] * last_r[k] * (last_r[k] * div_by(c[2 * k + 1], n, inv_n)));
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
-          if (!live(i)) continue;
           F2 d[kPairs], v[kPairs];
-          U::pairs(*slot(last_stage, k, 0, i), d);
-          U::pairs(*slot(last_stage, k, 1, i), v);
+          U::pairs(live(i) ? *slot(last_stage, k, 0, i) : no_unit(), d);
+          U::pairs(live(i) ? *slot(last_stage, k, 1, i) : no_unit(), v);
 #pragma unroll
           for (int j = 0; j < kPairs; ++j)
             v[j] = fma2(add2(v[j], minus_mu), k2, fma2(mul2(d[j], w[i][j]), rr, k1));
-          U::store_pairs(dxr + k * a.dx_stride + i * kTpr * kPer, v);
+          if (live(i)) U::store_pairs(dxr + k * a.dx_stride + i * kTpr * kPer, v);
         }
       }
       dxr += step * a.dx_stride;
@@ -1293,21 +1291,33 @@ void with_group(int64_t cols, F&& f) {
 
 template <class T>
 void launch_forward_stream(const ForwardArgs& a, cudaStream_t s) {
+  using std::integral_constant;
   constexpr int kUnits = 16 / Unit<T>::kPer;
   with_group(a.cols, [&](auto warps, auto blocks) {
     constexpr int kW = decltype(warps)::value, kC = decltype(blocks)::value;
-    const bool full = a.cols == 512 * kW * kC;
     const int64_t pairs = (a.rows + 1) / 2;
     if constexpr (kC > 1) {
-      constexpr int kRows = sizeof(T) == 2 ? 2 : 1, kStages = 5;
-      using S = Stream<T, kUnits, kW, 1, kStages, kRows>;
-      launch_stream<kC>(full ? layer_norm_cluster_kernel<T, kW, kC, kRows, kStages, true>
-                             : layer_norm_cluster_kernel<T, kW, kC, kRows, kStages, false>,
-                        a, kRows == 2 ? pairs : a.rows, S::kThreads, S::kSmem, s);
+      constexpr int kRows = sizeof(T) == 2 ? 2 : 1;
+      auto over = [&](auto elems, auto w, auto c, auto stages) {
+        constexpr int kElems = decltype(elems)::value, kWc = decltype(w)::value, kCc = decltype(c)::value;
+        constexpr int kStages = decltype(stages)::value;
+        using S = Stream<T, kElems / Unit<T>::kPer, kWc, 1, kStages, kRows>;
+        launch_stream<kCc>(a.cols == 32 * kElems * kWc * kCc
+                               ? layer_norm_cluster_kernel<T, kElems, kWc, kCc, kRows, kStages, true>
+                               : layer_norm_cluster_kernel<T, kElems, kWc, kCc, kRows, kStages, false>,
+                           a, kRows == 2 ? pairs : a.rows, S::kThreads, S::kSmem, s);
+      };
+      // 16384 .. 24576 columns: 24 elements to a thread of two blocks, not 16 of four, of which
+      // fewer fit (1600 x 20000 bf16 26.7 us against 40.5, f32 42.5 against 52.9)
+      if constexpr (kC == 4 && kW == 12)
+        over(integral_constant<int, 24>{}, integral_constant<int, 16>{}, integral_constant<int, 2>{},
+             integral_constant<int, 4>{});
+      else
+        over(integral_constant<int, 16>{}, warps, blocks, integral_constant<int, 5>{});
     } else if constexpr (sizeof(T) == 2) {
       constexpr int kGroups = kW == 1 ? 15 : 16 / kW, kStages = 3;
       using S = Stream<T, kUnits, kW, kGroups, kStages, 2>;
-      launch_stream<1>(full ? layer_norm_stream_kernel<T, kW, kGroups, kStages, true>
+      launch_stream<1>(a.cols == 512 * kW ? layer_norm_stream_kernel<T, kW, kGroups, kStages, true>
                             : layer_norm_stream_kernel<T, kW, kGroups, kStages, false>,
                        a, pairs, S::kThreads, S::kSmem, s);
     }
@@ -1316,11 +1326,13 @@ void launch_forward_stream(const ForwardArgs& a, cudaStream_t s) {
 
 // Which kernel, with kernel times of both sides (us):
 //   whole units, few rows   a row to 1, 4 or 16 warps, one unit to a thread where it fits:
-//                           1000 x 1024 f32 2.5, streamed 3.1
+//                           1000 x 1024 f32 2.5, streamed 3.1; of more than 2048 units
+//                           streamed: 400 x 17408 bf16 10.2, a row to 16 warps 12.5
 //   f32 up to 8192 columns  a row to 1, 2 or 4 warps: 16384 x 2048 42.3, streamed 47.9
 //   bf16, and wider f32     streamed: 8192 x 4096 bf16 22.4, a row to a warp 37.5; over
 //                           clusters: 4096 x 16384 bf16 43.6, a row to a block 99
-//   the rest up to 16384    element by element: 8192 x 4097 bf16 46, three reads 94
+//   the rest up to 16384    element by element: 8192 x 4097 bf16 46, three reads 94 (1600 x
+//                           17409 with 1024 threads: bf16 54, f32 66, three reads 49, 76)
 //   wider still             three reads
 template <class T>
 void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
@@ -1351,7 +1363,7 @@ void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
     row_kernel(integral_constant<int, 1>{}, integral_constant<int, 1>{});
   } else if (whole && few && n <= 128) {
     row_kernel(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-  } else if (whole && !few && (sizeof(T) == 2 || n > 2048) && a.cols <= kStreamCols) {
+  } else if (whole && ((!few && sizeof(T) == 2) || n > 2048) && a.cols <= kStreamCols) {
     launch_forward_stream<T>(a, s);
   } else if (whole && sizeof(T) == 4 && !few && n <= 512) {
     if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 1>{}, integral_constant<int, 16>{});

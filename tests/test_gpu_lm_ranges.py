@@ -64,6 +64,20 @@ def test_layer_norm_of_wide_odd_rows(rows, cols, dtype):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, cols", [(1, 16392), (2, 17408), (3, 24576), (75, 20000), (149, 20000), (400, 16400),
+                                        (30, 8200), (1, 12288), (33, 24584), (1, 32768), (599, 18440)])
+def test_layer_norm_of_few_wide_rows(rows, cols, dtype):
+    x, w, b, dy = ln._inputs(rows, cols, dtype, seed=cols + rows)
+    y, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    ln._check_forward(x, w, b, y, mean, rstd)
+    out = torch.full((rows, cols + 8), 7.0, dtype=dtype, device=DEV)
+    mcke.layer_norm(x, w, b, out=out[:, :cols])
+    assert torch.equal(out[:, :cols], y) and bool((out[:, cols:] == 7.0).all())
+    ln._check_backward(x, w, mean, rstd, dy, *mcke.layer_norm_backward(dy, x, mean, rstd, w))
+    mcke.check_device_errors()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows, cols, k", [(18, 200000, 32), (19, 200000, 32), (74, 131072, 9), (149, 70001, 8),
                                            (1184, 2048, 5), (1183, 2048, 5), (1500, 4096, 32), (1500, 4104, 32),
                                            (3000, 24, 20), (888, 40000, 0), (889, 40000, 1), (2, 1 << 22, 4)])
