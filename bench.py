@@ -1317,6 +1317,29 @@ def run_profile(args) -> None:
             b = torch.rand(n, n, generator=gen, device=dev) * 2 - 1
             c = torch.empty(n, n, device=dev)
             fn = lambda: mcke.gemm(a, b, c, variant="simt")  # noqa: E731
+        elif name == "layer_norm":
+            # forward and backward, 8192 rows of 4096 bf16
+            x, dy = (torch.randn(8192, 4096, generator=gen, device=dev).to(torch.bfloat16) for _ in range(2))
+            w, b = (torch.randn(4096, generator=gen, device=dev) for _ in range(2))
+
+            def fn(x=x, dy=dy, w=w, b=b):
+                _, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+                mcke.layer_norm_backward(dy, x, mean, rstd, w)
+        elif name == "token_logprobs":
+            # with the entropy, 4096 rows of 50257 bf16 logits, and their gradient
+            x = torch.randn(4096, 50257, generator=gen, device=dev, dtype=torch.bfloat16)
+            t = torch.randint(0, 50257, (4096,), generator=gen, device=dev)
+            g = torch.randn(4096, generator=gen, device=dev)
+            dx = torch.empty_like(x)
+
+            def fn(x=x, t=t, g=g, dx=dx):
+                r = mcke.token_logprobs(x, t, entropy=True)
+                mcke.token_logprobs_backward(x, r.lse, t, g, r.entropy, g, out=dx)
+        elif name == "clip_grads":
+            # 20 bf16 tensors of 16 M elements, clipped to half their norm
+            grads = [torch.randn(1 << 24, generator=gen, device=dev).to(torch.bfloat16) for _ in range(20)]
+            outs = [torch.empty_like(t) for t in grads]
+            fn = lambda grads=grads, outs=outs: mcke.clip_grad_norm(grads, 9e3, out=outs)  # noqa: E731
         elif name.startswith("reduce_timeline"):
             # Phase breakdown of the one-kernel sharded reduce at world 1
             # (reduce_timeline or reduce_timeline:<log2 n>): K steps back to
