@@ -372,7 +372,8 @@ int mcke_sm100_gemm_plan(int64_t m, int64_t n, int64_t k, int variant, int c_dty
 
 /* Layer norm of each row: y = (x - mean) * rstd * weight + bias with
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  weight and bias: [cols] or NULL
- * (1 and 0).  mean and rstd: [rows], what the backward pass takes, or NULL.
+ * (1 and 0).  mean and rstd: [rows], what the backward pass takes, or NULL (refused for
+ * rows of no columns).
  * eps finite and >= 0. */
 int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const float* weight, const float* bias, void* y,
                           int64_t y_stride, float* mean, float* rstd, int64_t rows, int64_t cols, float eps,

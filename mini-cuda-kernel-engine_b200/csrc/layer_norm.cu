@@ -1487,6 +1487,8 @@ extern "C" int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const floa
   MCKE_RETURN_IF(check_dtype(who, dtype));
   if (rows < 0 || cols < 0) return fail(MCKE_INVALID_ARGUMENT, "%s: negative extent", who);
   if (!(eps >= 0.0f) || std::isinf(eps)) return fail(MCKE_INVALID_ARGUMENT, "%s: eps must be finite and >= 0", who);
+  if (rows > 0 && cols == 0 && (mean || rstd))
+    return fail(MCKE_INVALID_ARGUMENT, "%s: rows of no columns have no statistics", who);
   if (rows == 0 || cols == 0) return MCKE_OK;
   if (!x || !y) return fail(MCKE_INVALID_ARGUMENT, "%s: null pointer", who);
   if (rows > kMaxRows || cols > 2147483647LL)

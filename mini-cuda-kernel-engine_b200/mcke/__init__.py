@@ -541,6 +541,12 @@ def _same(t, like: torch.Tensor, name: str) -> None:
                          f"{t.device}")
 
 
+def _workspace(t: torch.Tensor, like: torch.Tensor) -> None:
+    # bytes that are not all t's own (a view with gaps, an expanded one) are not workspace
+    if t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"workspace must be contiguous on {like.device}")
+
+
 def _elsewhere(t: torch.Tensor, stream) -> bool:
     """Whether a call has to switch to t's device or to ``stream`` first."""
     return stream is not None or torch.cuda.current_device() != t.get_device()
@@ -617,8 +623,8 @@ def layer_norm_backward(dy, x, mean, rstd, weight=None, out=None, param_grads: b
         dw, db = x.new_empty(cols, dtype=torch.float32), x.new_empty(cols, dtype=torch.float32)
         if workspace is None:
             workspace = x.new_empty(layer_norm_backward_workspace_bytes(rows, cols), dtype=torch.uint8)
-    if workspace is not None and workspace.device != x.device:
-        raise ValueError(f"workspace must be on {x.device}")
+    if workspace is not None:
+        _workspace(workspace, x)
     _check(lib().mcke_sm100_layer_norm_backward(
         dy.data_ptr(), dys, x.data_ptr(), xs, w, m, r, out.data_ptr(), dxs, _ptr(dw), _ptr(db), rows, cols,
         _DTYPE_OF[x.dtype], _ptr(workspace), 0 if workspace is None else workspace.nbytes, _current(x)))
@@ -652,12 +658,12 @@ def token_logprobs(logits, targets=None, top_k: int = 0, entropy: bool = False, 
     lp = None if targets is None else logits.new_empty(shape, dtype=torch.float32)
     ent = logits.new_empty(shape, dtype=torch.float32) if entropy else None
     top = ids = None
-    if top_k:
-        k = max(int(top_k), 0)  # the library refuses a negative one
+    k = min(max(int(top_k), -1), TOP_MAX + 1)  # the library refuses both ends
+    if k > 0:
         top = logits.new_empty((*shape, k), dtype=torch.float32)
         ids = logits.new_empty((*shape, k), dtype=torch.int64)
     _check(lib().mcke_sm100_token_logprobs(logits.data_ptr(), xs, rows, cols, _DTYPE_OF[logits.dtype], t, _ptr(lp),
-                                           lse.data_ptr(), _ptr(ent), top_k, _ptr(top), _ptr(ids), _current(logits)))
+                                           lse.data_ptr(), _ptr(ent), k, _ptr(top), _ptr(ids), _current(logits)))
     return TokenLogprobs(lp, lse, ent, top, ids)
 
 
@@ -731,8 +737,8 @@ def _norm_buffers(grads, norm, workspace):
         _one_float(norm, grads[0])
     if workspace is None:
         workspace = grads[0].new_empty(grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8)
-    elif workspace.device != grads[0].device:
-        raise ValueError(f"workspace must be on {grads[0].device}")
+    else:
+        _workspace(workspace, grads[0])
     return norm, workspace
 
 

@@ -198,3 +198,24 @@ def test_a_workspace_of_the_callers():
     assert torch.equal(mcke.grad_norm(grads, workspace=ws), mcke.grad_norm(grads))
     out = torch.zeros((), device=DEV)
     assert mcke.grad_norm(grads, norm=out) is out and out > 0
+
+
+def test_refusals_of_the_binding():
+    x, w, b, dy = ln._inputs(6, 64, F32, seed=1)
+    _, mean, rstd = mcke.layer_norm(x, w, b, save_stats=True)
+    need = mcke.layer_norm_backward_workspace_bytes(6, 64)
+    for ws in (torch.empty(1, dtype=torch.uint8, device=DEV).expand(need),  # one byte, listed need times
+               torch.empty(2 * need, dtype=torch.uint8, device=DEV)[::2], torch.empty(need, dtype=torch.uint8)):
+        with pytest.raises(ValueError, match="workspace"):
+            mcke.layer_norm_backward(dy, x, mean, rstd, w, workspace=ws)
+    need = mcke.grad_norm_workspace_bytes(1)
+    for f in (mcke.grad_norm, lambda g, workspace: mcke.clip_grad_norm(g, 1.0, workspace=workspace)):
+        with pytest.raises(ValueError, match="workspace"):
+            f([x], workspace=torch.empty(1, dtype=torch.uint8, device=DEV).expand(need))
+    for k in (33, 1 << 40, -1):
+        with pytest.raises(mcke.MckeError, match="top_k"):
+            mcke.token_logprobs(x, top_k=k)
+    with pytest.raises(mcke.MckeError, match="no statistics"):
+        mcke.layer_norm(x[:, :0], save_stats=True)
+    assert mcke.layer_norm(x[:, :0]).shape == (6, 0)
+    assert mcke.layer_norm(x[:0], save_stats=True)[1].shape == (0,)
