@@ -191,7 +191,7 @@ __device__ __forceinline__ void cluster_barrier() {
 constexpr int kMaxCluster = 8;
 constexpr int kLoads = 4;  // vectors of a thread in flight
 template <class T>
-constexpr int64_t kWarpCols = 32 * kLoads * 4 * Vec<T>::kPer;
+constexpr int64_t kWarpCols = 32 * kLoads * 4 * Vec<T>::kPer;  // four rounds of a warp
 
 // For the entropy 2^t t has to stay finite.  Next to a maximum in (kMaxAbove, kMaxBelow)
 // it is enough to raise the elements below kLow (-inf among them) to it, two bf16 at a
@@ -283,7 +283,9 @@ __device__ __forceinline__ void pick_chunks(const float* chunk_max, int chunks, 
 // from counting.  Only the k chunks are read again.  Their elements that the k-th
 // maximum does not rule out, a few more than k, are left in 32 places of their
 // warp and ranked; a warp that equal values give more than that keeps its k best in
-// its lanes instead.
+// its lanes instead.  With fewer chunks than k all of them are read again, twice: first
+// for each thread's own maximum, whose k-th rules elements out in the same way (1200 x
+// 4500 bf16, k = 20: 22.1 us, 51.8 with every element counted).
 template <class T, int kRowWarps, class Sync>
 __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift,
                                             const float* chunk_max, uint64_t* run_keys, int chunks, int k,
@@ -293,7 +295,13 @@ __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t 
   const int lane = threadIdx.x & 31, warp = kRowWarps == 1 ? 0 : threadIdx.x >> 5;
   const int t = kRowWarps == 1 ? lane : threadIdx.x;
   uint64_t key = 0;
-  if (kRowWarps > 1 && k <= kFewTop) {
+  if (chunks < k) {
+    float m = -INFINITY;
+    for (int c = warp; c < chunks; c += kRowWarps)
+      m = max_nan(m, vec_max(ld_row(row, (first_vec + static_cast<int64_t>(c) * 32 + lane) * kPer - shift, cols), row));
+    space.keys[t] = full_key(m, t);
+    k_largest(space.keys, kThreads, space.best, k, t, kThreads, sync);
+  } else if (kRowWarps > 1 && k <= kFewTop) {
     if (warp == 0) pick_chunks(chunk_max, chunks, k, space.best);
     sync();
   } else {
@@ -313,8 +321,7 @@ __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t 
     }
   }
   const int n = min(k, chunks);
-  // fewer chunks than k: all of their elements count
-  const float threshold = n < k ? -INFINITY : key_value(static_cast<uint32_t>(space.best[k - 1] >> 32));
+  const float threshold = key_value(static_cast<uint32_t>(space.best[k - 1] >> 32));
   // f(lanes whose element counts, the element's value, its index), for this warp's chunks
   auto for_candidates = [&](auto&& f) {
     for (int i0 = warp; i0 < n; i0 += kRowWarps * kBatch) {
@@ -323,7 +330,8 @@ __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t 
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (i0 + u * kRowWarps >= n) break;
-        first[u] = (first_vec + key_index(space.best[i0 + u * kRowWarps]) * 32 + lane) * kPer - shift;
+        const int64_t c = chunks < k ? i0 + u * kRowWarps : key_index(space.best[i0 + u * kRowWarps]);
+        first[u] = (first_vec + c * 32 + lane) * kPer - shift;
         q[u] = ld_row(row, first[u], cols);
       }
 #pragma unroll
@@ -682,11 +690,17 @@ int row_blocks(int64_t rows, int64_t cols) {
   }
   return best;
 }
-// A row to a warp where a block would have few rounds of loads for it and there are
-// rows enough for every SM's warps.
+// A row to a warp where a block would have few rounds of loads for it, up to 32 KB, if there
+// are rows enough for every SM's warps, the more the longer they are.  us, a warp against a
+// block: bf16 8000 x 5000 18.2, 39.5; 3000 x 8000 15.7, 15.5; 8000 x 16000 48.0, 53.1; 8192 x
+// 32768 98, 89; 1300 x 8000 9.9, 8.4; f32 8000 x 5000 28.4, 43.5; 1300 x 5000 10.5, 10.6; 8000
+// x 16000 87, 78.  More than a few alternatives keep a warp long, and only narrow
+// rows make up for it (4000 x 12000 bf16, k = 20: 58, 50).
 template <class T>
-bool warp_rows(int64_t rows, int64_t cols) {
-  return cols <= kWarpCols<T> && rows >= 148 * 8;
+bool warp_rows(int64_t rows, int64_t cols, int top_k) {
+  if (rows < 148 * 8) return false;
+  if (top_k > kFewTop) return cols <= kWarpCols<T>;
+  return cols <= 32768 / static_cast<int64_t>(sizeof(T)) && cols <= rows * (sizeof(T) == 2 ? 5 : 4);
 }
 
 template <class T, int kRowWarps, bool kTop>
@@ -726,7 +740,7 @@ void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t
 // are the faster (89 us against 94).
 template <class T>
 void launch_forward(const T* x, const ForwardArgs& a, int64_t rows, cudaStream_t s) {
-  const bool narrow = warp_rows<T>(rows, a.cols);
+  const bool narrow = warp_rows<T>(rows, a.cols, a.top_k);
   if (a.top_k == 0) narrow ? launch_forward<T, 1, false>(x, a, rows, s) : launch_forward<T, 8, false>(x, a, rows, s);
   else if (narrow) launch_forward<T, 1, true>(x, a, rows, s);
   else if (rows * kMaxCluster <= 148) launch_forward<T, 8, true>(x, a, rows, s);

@@ -91,6 +91,23 @@ def test_token_logprobs_by_size(rows, cols, k, dtype):
     lp._check_backward(x, t, r.lse, r.entropy, gl, ge, None, dx)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows, cols, k", [(1184, 5920, 8), (1184, 5921, 0), (1300, 4736, 1), (3277, 16384, 8), (3300, 16385, 8),
+                                           (8000, 4999, 3), (1200, 4500, 20), (5, 4500, 32), (1, 300, 32), (2000, 257, 9),
+                                           (3, 33, 32), (40, 8191, 31), (1200, 64, 32)])
+def test_token_logprobs_of_rows_to_a_warp(rows, cols, k, dtype):
+    x, t = lp._logits(rows, cols, dtype, seed=rows + cols, masked=0.02)
+    lp._check(x, t, mcke.token_logprobs(x, t, top_k=k, entropy=True), k)
+    if k:
+        # all equal, nothing but a few left, a NaN: the first of the equal come first
+        flat = torch.full((3, cols), 0.5, dtype=dtype, device=DEV)
+        flat[1, 2:] = float("-inf")
+        flat[2, cols // 2] = float("nan")
+        ids = mcke.token_logprobs(flat, top_k=k).top_ids
+        assert ids[0].tolist() == list(range(k)) and ids[1].tolist() == list(range(k))
+        assert ids[2].tolist() == [cols // 2] + [i for i in range(k) if i != cols // 2][: k - 1]
+
+
 def test_offsets_past_32_bits():
     stride = (1 << 31) + 24
     buf = torch.empty(2 * stride, dtype=BF16, device=DEV)
