@@ -94,7 +94,8 @@ def test_token_logprobs_by_size(rows, cols, k, dtype):
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows, cols, k", [(1184, 5920, 8), (1184, 5921, 0), (1300, 4736, 1), (3277, 16384, 8), (3300, 16385, 8),
                                            (8000, 4999, 3), (1200, 4500, 20), (5, 4500, 32), (1, 300, 32), (2000, 257, 9),
-                                           (3, 33, 32), (40, 8191, 31), (1200, 64, 32)])
+                                           (3, 33, 32), (40, 8191, 31), (1200, 64, 32), (300, 2560, 20),
+                                           (300, 2815, 20), (1300, 5632, 20), (90, 5633, 20), (70, 1152, 8), (1200, 2304, 8)])
 def test_token_logprobs_of_rows_to_a_warp(rows, cols, k, dtype):
     x, t = lp._logits(rows, cols, dtype, seed=rows + cols, masked=0.02)
     lp._check(x, t, mcke.token_logprobs(x, t, top_k=k, entropy=True), k)
