@@ -374,14 +374,19 @@ int mcke_sm100_gemm_plan(int64_t m, int64_t n, int64_t k, int variant, int c_dty
  * rstd = 1 / sqrt(mean((x - mean)^2) + eps).  weight and bias: [cols] or NULL
  * (1 and 0).  mean and rstd: [rows], what the backward pass takes, or NULL (refused for
  * rows of no columns).
- * eps finite and >= 0. */
+ * eps finite and >= 0.
+ * A sum past float32's range is infinite: a row that holds an infinity, or whose
+ * values add up past the range, gets an infinite mean (NaN where both signs meet)
+ * and NaN for y; one whose squared deviations do gets rstd 0 and y = bias. */
 int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const float* weight, const float* bias, void* y,
                           int64_t y_stride, float* mean, float* rstd, int64_t rows, int64_t cols, float eps,
                           int dtype, mcke_stream_t stream);
 /* The backward pass.  With xh = (x - mean) * rstd and g = dy * weight:
  * dx = rstd * (g - mean(g) - xh * mean(g * xh)), dweight = the sum over rows of
  * dy * xh, dbias = the sum over rows of dy.  dweight and dbias: [cols] or NULL
- * (with both NULL no workspace is needed).  rows == 0 writes zeros to them. */
+ * (with both NULL no workspace is needed).  rows == 0 writes zeros to them.  A row
+ * with rstd 0 has dx = 0 and adds nothing to dweight (where dy * (x - mean) is in
+ * float32's range). */
 size_t mcke_sm100_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
 int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
                                    const float* weight, const float* mean, const float* rstd, void* dx,

@@ -745,6 +745,11 @@ __device__ __forceinline__ bool join_groups(F2* cell, int group, F2* dw, F2* db)
   return true;
 }
 
+// What x - mu is multiplied by in dx: -r^2 c2, where c2 is r times `c`, the mean of dy w
+// (x - mu).  A row whose squared deviations are past float's range has r = 0 and takes no
+// part, though `c` may be infinite.
+__device__ __forceinline__ float dx_scale(float r, float c) { return r == 0.0f ? 0.0f : -r * r * (r * c); }
+
 // dx, and the column sums of each slab (the rows of one cluster), in one read of dy
 // and x: a thread adds up its 16 columns in registers over all its rows, the
 // block's groups are added in shared memory at the end.  Each turn of the loop
@@ -868,10 +873,10 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_kern
 #pragma unroll
       for (int k = 0; k < kRows; ++k) {
         if (kRows > 1 && row - step + k >= a.rows) break;
-        // dx = r dy w - r c1 - (x - mu) r^2 c2, the second sum being r short of c2's
+        // dx = r dy w - r c1 - (x - mu) r^2 c2
         const F2 minus_mu = f2(-last_mu[k]), rr = f2(last_r[k]);
         const F2 k1 = f2(-last_r[k] * div_by(c[2 * k], n, inv_n));
-        const F2 k2 = f2(-last_r[k] * last_r[k] * (last_r[k] * div_by(c[2 * k + 1], n, inv_n)));
+        const F2 k2 = f2(dx_scale(last_r[k], div_by(c[2 * k + 1], n, inv_n)));
 #pragma unroll
         for (int i = 0; i < kUnits; ++i) {
           F2 d[kPairs], v[kPairs];
@@ -1031,7 +1036,7 @@ __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elem
       collect_sums(c, posted[group], (turn - 1) % kPlaces, static_cast<uint32_t>((turn - 1) / kPlaces) & 1u);
       const F2 minus_mu = f2(-last_mu), rr = f2(last_r);
       const F2 k1 = f2(-last_r * div_by(c[0], n, inv_n));
-      const F2 k2 = f2(-last_r * last_r * (last_r * div_by(c[1], n, inv_n)));
+      const F2 k2 = f2(dx_scale(last_r, div_by(c[1], n, inv_n)));
       T* dx = static_cast<T*>(a.dx) + static_cast<int64_t>(row - step) * a.dx_stride;
       for_units(last_stage, [&](int i, const auto& d, const auto& v) {
 #pragma unroll

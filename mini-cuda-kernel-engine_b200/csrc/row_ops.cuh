@@ -3,6 +3,7 @@
 // points (row strides, overlap of outputs with inputs).
 #pragma once
 
+#include <cfloat>
 #include <cmath>
 #include <initializer_list>
 
@@ -138,10 +139,11 @@ __device__ __forceinline__ float sum2(F2 a) {
 }
 
 // s / n for a row length n whose reciprocal is at hand: the product, and
-// Markstein's correction of it by the remainder.
+// Markstein's correction of it by the remainder.  Of an infinite q the remainder is a
+// NaN, of which fmaxf makes a finite number, and q stays as it is.
 __device__ __forceinline__ float div_by(float s, float n, float inv_n) {
   const float q = s * inv_n;
-  return fmaf(fmaf(-q, n, s), inv_n, q);
+  return fmaf(fmaxf(fmaf(-q, n, s), -FLT_MAX), inv_n, q);
 }
 
 // ---- device: sums --------------------------------------------------------------------
