@@ -502,7 +502,8 @@ def gemm_f32_tc(a, b, c=None, alpha: float = 1.0, beta: float = 0.0, bias=None, 
 # ---- operators of language models ----------------------------------------------------
 #
 # These calls run on the tensors' device whether or not it is the current one.
-# With an explicit ``stream`` what a call allocates belongs to that stream.
+# With an explicit ``stream``, which has to be of that device, what a call allocates
+# belongs to that stream.
 
 _DTYPE_OF = {torch.float32: DTYPE["f32"], torch.bfloat16: DTYPE["bf16"]}
 
@@ -557,6 +558,8 @@ def _elsewhere(t: torch.Tensor, stream) -> bool:
 def _on(t: torch.Tensor, stream):
     """t's device, and ``stream`` (a torch stream, or a raw handle), made current: launches
     reach them and allocations belong to them."""
+    if hasattr(stream, "cuda_stream") and stream.device.index != t.get_device():
+        raise ValueError(f"stream is on {stream.device}, the tensors on {t.device}")
     with torch.cuda.device(t.device):
         if stream is None:
             yield
