@@ -392,6 +392,10 @@ int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride, const void
                                    const float* weight, const float* mean, const float* rstd, void* dx,
                                    int64_t dx_stride, float* dweight, float* dbias, int64_t rows, int64_t cols,
                                    int dtype, void* workspace, size_t workspace_bytes, mcke_stream_t stream);
+/* Like mcke_sm100_watchdog_selftest, of the wait in which both passes collect a row's
+ * sums: enqueues a kernel of one block in which it runs out (after 20 ms instead
+ * of 2 s), so that the next mcke_sm100_check_device_errors() names the layer norm. */
+int mcke_sm100_layer_norm_watchdog_selftest(mcke_stream_t stream);
 
 /* Of each row of logits: logprobs = the log probability of its target,
  * lse = log(sum(exp)), entropy = -sum(p log p) (natural logarithms), and the

@@ -163,7 +163,7 @@ extern "C" int mcke_sm100_check_device_errors(mcke_stream_t stream) {
                 "reduce (one-kernel step): a CTA's partial did not arrive within 1 s; the result is incomplete");
   MCKE_RETURN_IF(read_layer_norm_watchdog(&site));
   if (site != 0)
-    return fail(MCKE_INTERNAL, "layer norm (backward): a row's sums did not arrive within 2 s; the result is incomplete");
+    return fail(MCKE_INTERNAL, "layer norm: a row's sums did not arrive in time; the result is incomplete");
   return MCKE_OK;
 }
 

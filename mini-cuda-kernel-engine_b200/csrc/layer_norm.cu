@@ -532,14 +532,15 @@ __device__ __forceinline__ bool try_phase(uint32_t bar, uint32_t phase) {
   return done != 0;
 }
 
-// Waits, 2 s at most: a wait that runs out is recorded and passed, as are all later ones
-// of the group, whose sums are then incomplete.
+// Waits, kLimitNs at most: a wait that runs out is recorded and passed, as are all later
+// ones of the group, whose sums are then incomplete.
+template <unsigned long long kLimitNs>
 __device__ __noinline__ void wait_phase(uint32_t bar, uint32_t phase, volatile int* gave_up) {
   unsigned long long t0, t;
   asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
   while (!*gave_up && !try_phase(bar, phase)) {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (t - t0 > kWaitNs) {
+    if (t - t0 > kLimitNs) {
       *gave_up = 1;
       atomicCAS(&g_layer_norm_watchdog, 0u, 1u);
     }
@@ -548,10 +549,10 @@ __device__ __noinline__ void wait_phase(uint32_t bar, uint32_t phase, volatile i
 
 // Waits until every share of place k is there, and returns the sums: the
 // same bits in every thread.
-template <int kN, int kW, int kCluster>
+template <unsigned long long kLimitNs = kWaitNs, int kN, int kW, int kCluster>
 __device__ __forceinline__ void collect_sums(float (&v)[kN], PostedSums<kN, kW, kCluster>& p, int k, uint32_t phase) {
   const uint32_t bar = shared_address(&p.arrived[k]);
-  if (!try_phase(bar, phase)) wait_phase(bar, phase, &p.gave_up);
+  if (!try_phase(bar, phase)) wait_phase<kLimitNs>(bar, phase, &p.gave_up);
   using P = PostedSums<kN, kW, kCluster>;
   const int lane = threadIdx.x & 31, at = (lane & 7) * P::kPerLane;
   const float* mine = p.share[k][(lane >> 3) % kN] + at;
@@ -563,6 +564,21 @@ __device__ __forceinline__ void collect_sums(float (&v)[kN], PostedSums<kN, kW, 
   for (int o = 4; o > 0; o >>= 1) a += __shfl_xor_sync(0xffffffffu, a, o);
 #pragma unroll
   for (int i = 0; i < kN; ++i) v[i] = __shfl_sync(0xffffffffu, a, 8 * i);
+}
+
+// Self-test of the wait: of a group's two warps one posts and the other does not.  The first
+// wait runs out after 20 ms and is recorded; the second could not end either and is passed.
+__global__ void __launch_bounds__(64) layer_norm_selftest_kernel() {
+  pdl_entry();
+  __shared__ PostedSums<2, 2, 1> posted;
+  if (threadIdx.x == 0) init_sums(posted);
+  __syncthreads();
+  if (threadIdx.x >= 32) return;
+  for (int k = 0; k < 2; ++k) {
+    float v[2] = {0.0f, 0.0f};
+    post_sums(v, posted, k);
+    collect_sums<20000000ull>(v, posted, k, 0);
+  }
 }
 
 // Rows over the blocks of a cluster.  The statistics take two exchanges, the mean's and
@@ -1515,7 +1531,7 @@ bool allow_shared_memory(const void* kernel, std::size_t bytes) {
   }
 }
 
-// Reads and clears the word that an expired wait of the backward pass sets.
+// Reads and clears the word that an expired wait of either pass sets.
 int read_layer_norm_watchdog(uint32_t* site) {
   uint32_t v = 0;
   cudaError_t e = cudaMemcpyFromSymbol(&v, g_layer_norm_watchdog, sizeof(v));
@@ -1531,6 +1547,12 @@ int read_layer_norm_watchdog(uint32_t* site) {
 }  // namespace mcke_sm100
 
 using namespace mcke_sm100;
+
+extern "C" int mcke_sm100_layer_norm_watchdog_selftest(mcke_stream_t stream) {
+  clear_error();
+  launch_async(layer_norm_selftest_kernel, 1, 64, 0, reinterpret_cast<cudaStream_t>(stream));
+  return check_launch("mcke_sm100_layer_norm_watchdog_selftest");
+}
 
 extern "C" int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const float* weight, const float* bias, void* y,
                                      int64_t y_stride, float* mean, float* rstd, int64_t rows, int64_t cols, float eps,

@@ -108,6 +108,7 @@ def lib() -> ctypes.CDLL:
             "mcke_sm100_layer_norm_backward_workspace_bytes": (sz, [i64, i64]),
             "mcke_sm100_layer_norm_backward": (i32, [vp, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, i64, i64, i32, vp,
                                                      sz, vp]),
+            "mcke_sm100_layer_norm_watchdog_selftest": (i32, [vp]),
             "mcke_sm100_token_logprobs": (i32, [vp, i64, i64, i64, i32, vp, vp, vp, vp, i32, vp, vp, vp]),
             "mcke_sm100_token_logprobs_backward": (i32, [vp, i64, i64, i64, i32, vp, vp, vp, vp, vp, vp, vp, i64,
                                                          vp]),
