@@ -1410,10 +1410,10 @@ void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
   const unsigned rows = static_cast<unsigned>(a.rows);
   const bool few = a.rows <= kFewRows;
   const int64_t n = a.cols / kPer;  // units
-  // a row's kW warps hold it at up to kMax units a thread
-  auto row_kernel = [&](auto w, auto max) {
+  // a row's kW warps hold it at kMin to kMax units a thread
+  auto row_kernel = [&](auto w, auto min, auto max) {
     constexpr int kW = decltype(w)::value;
-    with_units<decltype(max)::value>(n, 32 * kW, [&](auto units, auto full) {
+    with_units<decltype(max)::value, decltype(min)::value>(n, 32 * kW, [&](auto units, auto full) {
       launch_async(layer_norm_kernel<T, decltype(units)::value, kW, decltype(full)::value>,
                    kW == 1 ? (rows + kWarps - 1) / kWarps : rows, kW == 1 ? kThreads : 32 * kW, 0, s, a);
     });
@@ -1429,19 +1429,22 @@ void launch_forward(const ForwardArgs& a, bool whole, cudaStream_t s) {
   } else if (!whole && a.cols <= 16384) {
     elements(integral_constant<int, 512>{}, integral_constant<int, 16>{});
   } else if (whole && few && n <= 32) {
-    row_kernel(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    row_kernel(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
   } else if (whole && few && n <= 128) {
-    row_kernel(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+    row_kernel(integral_constant<int, 4>{}, integral_constant<int, 1>{}, integral_constant<int, 1>{});
   } else if (whole && ((!few && sizeof(T) == 2) || n > 2048) && a.cols <= kStreamCols) {
     launch_forward_stream<T>(a, s);
   } else if (whole && sizeof(T) == 4 && !few && n <= 512) {
-    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 1>{}, integral_constant<int, 16>{});
+    if constexpr (sizeof(T) == 4)
+      row_kernel(integral_constant<int, 1>{}, integral_constant<int, 1>{}, integral_constant<int, 16>{});
   } else if (whole && sizeof(T) == 4 && !few && n <= 1024) {
-    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 2>{}, integral_constant<int, 16>{});
+    if constexpr (sizeof(T) == 4)
+      row_kernel(integral_constant<int, 2>{}, integral_constant<int, 16>{}, integral_constant<int, 16>{});
   } else if (whole && sizeof(T) == 4 && !few && n <= 2048) {
-    if constexpr (sizeof(T) == 4) row_kernel(integral_constant<int, 4>{}, integral_constant<int, 16>{});
-  } else if (whole && n <= 4096) {
-    row_kernel(integral_constant<int, 16>{}, integral_constant<int, 8>{});
+    if constexpr (sizeof(T) == 4)
+      row_kernel(integral_constant<int, 4>{}, integral_constant<int, 16>{}, integral_constant<int, 16>{});
+  } else if (whole && n <= 2048) {
+    row_kernel(integral_constant<int, 16>{}, integral_constant<int, 1>{}, integral_constant<int, 4>{});
   } else {
     launch_async(layer_norm_row_kernel<T>, rows, kThreads, 0, s, static_cast<const T*>(a.x), a.x_stride, a.weight,
                  a.bias, static_cast<T*>(a.y), a.y_stride, a.mean, a.rstd, static_cast<int64_t>(a.cols), a.eps);
