@@ -367,7 +367,8 @@ int mcke_sm100_gemm_plan(int64_t m, int64_t n, int64_t k, int variant, int c_dty
  * one buffer do not).  A workspace is written before it is read, need not be
  * cleared and must not be shared by calls that may run at the same time (two
  * captured graphs on two streams, for instance).  Results have the same bits on
- * every run.  All calls may be captured into a CUDA graph.  The stream belongs to
+ * every run with the same extents, strides and alignment of the tensors (which
+ * choose the kernel, and with it the order of sums).  All calls may be captured into a CUDA graph.  The stream belongs to
  * the current device. */
 
 /* Layer norm of each row: y = (x - mean) * rstd * weight + bias with
@@ -416,6 +417,7 @@ int mcke_sm100_token_logprobs(const void* logits, int64_t stride, int64_t rows, 
  * of them NULL, not all): with p = exp(logits - lse),
  * dlogits_j = grad_logprobs * ([j = target] - p_j)
  *             - grad_entropy * p_j * (log p_j + entropy) + grad_lse * p_j.
+ * A p_j below float32's smallest normal number counts as 0.
  * lse and entropy are the forward pass's (entropy only with grad_entropy,
  * targets only with grad_logprobs).  A row of -inf alone gets zeros; a negative
  * target takes no part in grad_logprobs, one >= cols gives NaN.  dlogits may be

@@ -954,7 +954,8 @@ __device__ __forceinline__ void pack_units(const uint16_t (&e)[16], uint4 (&q)[2
 // units: a thread reads only its own.  Bound by the element-wide accesses: 8192 x 4097
 // bf16 85 us (2.37 TB/s, 0.36 of the copy rate; 98 with elements in the ring, 142 with a pass
 // each for dx and for the sums), 5003 x 1537 f32 26 us (0.54); over clusters 2000 x 20001 bf16
-// 119 us, the two passes 195.
+// 119 us, the two passes 195.  Some instances spill, the f32 one over four blocks most (60
+// bytes stored, 104 loaded), the others 8 and less.
 template <class T, int kW, int kGroups, int kCluster>
 __global__ void __launch_bounds__(32 * kW * kGroups, 1) layer_norm_backward_elements_kernel(const BackwardArgs a) {
   pdl_entry();
@@ -1281,8 +1282,8 @@ bool whole_units(std::initializer_list<const void*> tensors, std::initializer_li
 // row is then spread over as many threads as it has units.
 constexpr int64_t kFewRows = 4 * 148;
 
-// Slabs of rows whose column sums are kept apart.  From the extents alone, so
-// the order of the sums, and every bit of dw and db, is the same on any GPU.
+// Slabs of rows whose column sums are kept apart: the same on any GPU, as is the kernel that
+// extents, strides and alignment choose, and so is every bit of dw and db.
 int64_t column_slabs(int64_t rows) { return rows < kStreamBlocks ? rows : kStreamBlocks; }
 
 // Calls f with the smallest of the unit counts kUnits, 2 kUnits .. kMax that holds n

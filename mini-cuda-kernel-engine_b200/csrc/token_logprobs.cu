@@ -286,7 +286,10 @@ __device__ __forceinline__ void pick_chunks(const float* chunk_max, int chunks, 
 // its lanes instead.  Where there are hardly more chunks than k their k-th maximum rules out
 // little, and all of them are read again, twice: first for each thread's own maximum, whose
 // k-th rules out more (1200 rows, k = 20: 2500 f32, 20 chunks, 19.1 us against 30.4; 5888
-// bf16, 23 chunks, 23.2 against 20.0).
+// bf16, 23 chunks, 23.2 against 20.0).  The border holds for k = 20 only: with fewer
+// alternatives threads' maxima win at more chunks than it says (8000 x 4000 bf16, k = 13,
+// 16 chunks of one warp, 48.6 us against the 62 taken; 1200 x 1400 f32, k = 9, 11 chunks, 10.9
+// against 14).
 template <class T, int kRowWarps, class Sync>
 __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t first_vec, int shift,
                                             const float* chunk_max, uint64_t* run_keys, int chunks, int k,
@@ -411,7 +414,8 @@ __device__ __forceinline__ void top_of_part(const T* row, int64_t cols, int64_t 
 // One read of the row: a warp has kLoads chunks in flight, takes their maximum, and
 // adds up the sums on its scale.  f32 is bound by HBM (4096 x 32768 80 us, 6.7 TB/s, 1.02 of
 // the copy rate: reads alone), bf16 by issue, the exponential unit 65% busy (8192 x
-// 32768 88.9 us, 6.04 TB/s, 0.92); with alternatives by a row's end, in which most warps
+// 32768 88.9 us, 6.04 TB/s, 0.92; 103 us in seconds of such calls, at the 1.65 GHz that the power
+// limit leaves of 1.965); with alternatives by a row's end, in which most warps
 // wait (the same rows with five 118 us).  One row of 131072: 10 us, of which 2 read it.
 template <int kRowWarps>
 constexpr int kBlockWarps = kRowWarps == 1 ? 4 : kRowWarps;
@@ -587,9 +591,12 @@ struct Grads {
 // `threads` threads of a block (a power of two) take a part of a row, kVecs vectors
 // each; kSame: dx has the row's offset from a 16-byte boundary, so whole vectors
 // are stored.
-// Bound by HBM: 4096 x 50257 bf16 with the entropy's gradient 136 us (6.04 TB/s, 0.92 of
-// the copy rate), 2048 x 32768 f32 80 us (1.02).  A check for whole blocks of vectors costs
-// more in registers than it saves (144 us).
+// A p below float's smallest normal number, 2^-126, is 0.
+// f32 is bound by HBM (2048 x 32768 80 us, 1.02 of the copy rate), bf16 by issue, 77% of
+// the slots (4096 x 50257 with the entropy's gradient 136 us, 6.04 TB/s, 0.92; 154 us in
+// seconds of such calls, at 1.63 GHz under the power limit).  Six blocks an SM leave 40
+// registers, of which the bf16 instances spill 12 to 40 bytes.  A check for whole blocks of
+// vectors costs more in registers than it saves (144 us).
 constexpr int kVecs = 4;
 template <class T, bool kEntropy, bool kSame>
 __global__ void __launch_bounds__(kThreads, 6)
@@ -675,11 +682,13 @@ __global__ void __launch_bounds__(kThreads, 6)
 // Blocks that share a row: 1, 2, 4 or 8, whichever takes the least time in rounds of
 // loads when the blocks run in waves over the device, with kTail rounds for what
 // a block does besides its loads.  With few rows that spreads a row over eight
-// blocks; with many it keeps the last wave from running half empty.
+// blocks; with many it keeps the last wave from running half empty.  The waves are counted
+// at the 40 registers of the kernels without alternatives; those with alternatives have 48 to
+// 64 and fit 32 to 40 warps an SM, not 48.
 template <class T, int kRowWarps, bool kTop>
 int row_blocks(int64_t rows, int64_t cols) {
   constexpr int64_t kRound = 32 * kRowWarps * kLoads * Vec<T>::kPer, kTail = kTop ? 4 : 2;
-  constexpr int64_t kResident = 148 * (48 / kRowWarps);  // at 40 registers a thread
+  constexpr int64_t kResident = 148 * (48 / kRowWarps);
   const int64_t rounds = (cols + kRound - 1) / kRound;
   int best = 1;
   int64_t best_time = 0;
