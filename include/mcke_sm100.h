@@ -387,7 +387,8 @@ int mcke_sm100_layer_norm(const void* x, int64_t x_stride, const float* weight, 
  * dy * xh, dbias = the sum over rows of dy.  dweight and dbias: [cols] or NULL
  * (with both NULL no workspace is needed).  rows == 0 writes zeros to them.  A row
  * with rstd 0 has dx = 0 and adds nothing to dweight (where dy * (x - mean) is in
- * float32's range). */
+ * float32's range).  dweight and dbias are float32 sums over a 148th of the rows each
+ * (a 74th from 8193 columns on, a 32nd from 16385 to 32768), joined in a fixed order. */
 size_t mcke_sm100_layer_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
 int mcke_sm100_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride,
                                    const float* weight, const float* mean, const float* rstd, void* dx,
